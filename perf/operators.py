@@ -87,7 +87,7 @@ def draw(rng):
         layer = rng.random() < 0.5
         case = _norm("", op, dtype, rows, cols, norm="layer" if layer else "rms", branch=branch, post=post, pre=pre,
                      bias=layer and (post or pre), groups=rng.choice([0] + divisors) if branch else 0,
-                     alpha=rng.choice([1.0, round(rng.uniform(0.5, 3.0), 2)]),
+                     alpha=rng.choice([1.0, round(rng.uniform(0.5, 3.0), 2)]) if branch else 1.0,
                      p=rate if branch and rng.random() < 0.5 else 0.0, params=rng.choice(["f32", dtype]))
     else:
         both, buckets = rng.random() < 0.6, rng.choice([16, 32, 64])
