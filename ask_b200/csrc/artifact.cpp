@@ -364,6 +364,14 @@ Generated generate(const ask_b200_plan& pl, const std::string& entry, const uint
       fail(ASK_B200_E_UNSUPPORTED,
            "scatter_add reads its base through the Runtime's pre_copy, which an external artifact cannot declare; "
            "run it as a recipe step");
+    case FAM_DROPOUT:
+    case FAM_BLOCK_NORM:
+    case FAM_BLOCK_NORM_GRAD:
+    case FAM_BIAS_SOFTMAX:
+    case FAM_BIAS_SOFTMAX_GRAD:
+      fail(ASK_B200_E_UNSUPPORTED,
+           "the training-block families (dropout, block_norm, bias_softmax and their gradients) are not lowered from an "
+           "ASK step, so there is no external kernel to package; run them as recipe steps");
     default:
       fail(ASK_B200_E_UNSUPPORTED, "the fused softmax is a runtime fusion; package its three steps instead");
   }

@@ -13,30 +13,13 @@
 #include <cuda_runtime.h>
 
 #include "kernels.h"
+#include "philox.cuh"
 
 namespace askb {
 
 namespace {
 
 constexpr int kGenThreads = 256;
-
-struct Philox {
-  uint32_t c[4];
-};
-
-__device__ __forceinline__ Philox philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0,
-                                               uint32_t k1) {
-  constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u, kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
-#pragma unroll
-  for (int round = 0; round < 10; ++round) {
-    const uint32_t hi0 = __umulhi(kM0, c0), lo0 = kM0 * c0;
-    const uint32_t hi1 = __umulhi(kM1, c2), lo1 = kM1 * c2;
-    const uint32_t n0 = hi1 ^ c1 ^ k0, n2 = hi0 ^ c3 ^ k1;
-    c0 = n0; c1 = lo1; c2 = n2; c3 = lo0;
-    k0 += kW0; k1 += kW1;
-  }
-  return Philox{{c0, c1, c2, c3}};
-}
 
 __global__ void __launch_bounds__(kGenThreads) gen_kernel(int kind, uint64_t seed, uint32_t sid, uint64_t offset,
                                                           uint64_t count, double p0, double p1,

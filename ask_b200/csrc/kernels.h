@@ -188,6 +188,107 @@ cudaError_t softmax_rows_launch(const SoftmaxArgs& a, int sms, cudaStream_t stre
 // one CTA per row); needs the device current.
 int softmax_rows_grid(const SoftmaxArgs& a, int sms);
 
+// ---- training-block operators: dropout, block norms, bucketed-bias softmax -------------
+// One dropout site: elements whose random word is below `threshold` =
+// floor(p * 2^32) are dropped, the others scaled by `scale` = 1 / (1 - p).
+struct DropSite {
+  uint32_t on, threshold, stream;
+  float scale;
+};
+
+// y = dropout(x) (+ residual), `count` contiguous elements (dropout_kernels.cu).
+struct DropoutArgs {
+  const void* x;
+  const void* residual;  // null: none
+  const int64_t* seed;   // {seed, offset} on the device
+  void* y;
+  uint64_t count;
+  int type;
+  DropSite drop;
+};
+cudaError_t dropout_launch(const DropoutArgs& a, int grid, cudaStream_t stream);
+cudaError_t dropout_occupancy(int type, bool residual, int* blocks_per_sm);
+constexpr int kDropThreads = 256;
+
+// How a row's threads are laid out: see row_team.cuh.
+struct TeamShape {
+  int warp_teams;  // every warp takes a row of its own
+  int threads;     // of a CTA
+  int ctas;        // of a row's cluster (1: no cluster)
+  int elems;       // row elements a thread holds
+};
+
+// Block norms (norm_kernels.cu).  Forward: h = alpha x + D(gate * N_post(y)),
+// u = N_pre(h); gradient: see the kernel.  x, y, h, u and the gradients to
+// them are [rows, cols] of `type`; weights, biases [cols] and gate
+// [groups, cols] of `ptype`; statistics [rows, 1 or 2] and the gradients to
+// the parameters f32.
+struct NormArgs {
+  const void *x, *y, *w_post, *b_post, *gate, *w_pre, *b_pre;
+  const int64_t* seed;
+  void *h, *u;
+  float *stats_post, *stats_pre;
+  // gradient
+  const void *dh, *du, *h_in;
+  const float *stats_post_in, *stats_pre_in;
+  void *dx, *dy;
+  float *dw_post, *db_post, *dgate, *dw_pre, *db_pre;
+  float* partial;  // [sum kinds][groups * chunks][cols]
+  uint64_t rows, rows_per_group;
+  uint32_t cols, groups, chunks;  // chunks of a group's rows, one team each (gradient)
+  float alpha, eps;
+  int type, ptype;
+  int branch, post, pre, layer, bias, gated;
+  DropSite drop;
+  TeamShape shape;
+};
+constexpr int kNormMaxCols = 32768;
+TeamShape norm_shape(uint64_t cols, bool grad);
+// Row sums the gradient keeps for each column: of B*yhat, B, du*hhat, du.
+struct NormSums {
+  bool t, s, p, q;
+  int count() const { return int(t) + int(s) + int(p) + int(q); }
+};
+NormSums norm_sums(const NormArgs& a);
+cudaError_t norm_occupancy(const NormArgs& a, bool grad, int* blocks_per_sm);
+cudaError_t norm_launch(const NormArgs& a, bool vec, int grid, cudaStream_t stream);
+cudaError_t norm_grad_launch(const NormArgs& a, bool vec, cudaStream_t stream);
+
+// Softmax over biased scores (bias_softmax_kernels.cu).  s, p, dp, ds are
+// [batch, heads, queries, keys] of `type`, table [buckets, heads] of
+// `table_type`, lengths and offsets i32 [batch] (null: all keys, 0), lse
+// [batch, heads, queries] f32.
+constexpr int kBiasMaxThresholds = 255;
+constexpr int kBiasMaxDistance = 4096;
+constexpr uint64_t kBiasMaxKeys = 131072;
+constexpr int kBiasMaxRowPerCta = 512 * 32;  // elements of a row that one CTA's registers hold
+struct BiasSoftmaxArgs {
+  const void *s, *dp, *table;
+  const float* lse_in;
+  const int *lengths, *offsets;
+  const int64_t* seed;
+  void* out;       // p, or ds
+  float* lse;      // forward
+  float* dtable;   // gradient, [buckets, heads]
+  float* partial;  // gradient: [heads * chunks * ctas][buckets]
+  uint64_t batch, queries;
+  uint32_t heads, keys, chunks;  // chunks of a head's (batch, query) pairs
+  uint32_t buckets;
+  float scale;
+  int type, table_type;
+  int causal, bidirectional, aligned;
+  int n_thresholds;
+  int thresholds[kBiasMaxThresholds];  // not falling; the bucket of a distance n is the number of them <= n
+  DropSite drop;
+  TeamShape shape;
+  uint32_t shared_bytes;
+};
+TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, int sms);
+// Threads of a CTA as the windows in shared memory allow, and those bytes.
+void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad);
+cudaError_t bias_softmax_occupancy(const BiasSoftmaxArgs& a, bool grad, int* blocks_per_sm);
+cudaError_t bias_softmax_launch(const BiasSoftmaxArgs& a, bool grad, cudaStream_t stream);
+
 cudaError_t gen_launch(int kind, uint64_t seed, uint32_t stream_id, uint64_t offset, uint64_t count, double p0,
                        double p1, const double* zipf_cdf, uint64_t zipf_n, void* dst, cudaStream_t stream);
 

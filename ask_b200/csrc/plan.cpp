@@ -400,7 +400,12 @@ void assign_registers(Program& p) {
 }
 
 // ---- plan -------------------------------------------------------------------------
-const char* const kFamilyNames[] = {"elementwise", "reduce", "gather", "scatter_add", "softmax"};
+const char* const kFamilyNames[] = {"elementwise", "reduce",     "gather",          "scatter_add",  "softmax",
+                                    "dropout",     "block_norm", "block_norm_grad", "bias_softmax", "bias_softmax_grad"};
+
+// The families whose kernels give a row (or a unit of elements) to threads in
+// their own way: their plans carry the CTA size in `block`.
+bool row_family(int family) { return family >= FAM_SOFTMAX; }
 
 uint64_t checked_count(const json::Value& v, const char* what) {
   const int64_t x = v.as_int(what);
@@ -849,6 +854,264 @@ void build_softmax(ask_b200_plan& pl, const json::Value& r) {
   pl.block = int(a.cols / 8 / uint64_t(vpt));
 }
 
+// ---- training-block operators -------------------------------------------------------
+double number_field(const json::Value& r, const char* key, double fallback) {
+  const json::Value* v = r.get(key);
+  if (!v) return fallback;
+  if (v->kind != json::Value::Number) fail(ASK_B200_E_INVALID, std::string(key) + " must be a number");
+  return v->num;
+}
+
+bool bool_field(const json::Value& r, const char* key, bool fallback) {
+  const json::Value* v = r.get(key);
+  if (!v) return fallback;
+  if (v->kind != json::Value::Bool) fail(ASK_B200_E_INVALID, std::string(key) + " must be true or false");
+  return v->b;
+}
+
+int activation_type(const json::Value& r) {
+  const int t = parse_dtype(r.at("dtype").as_str("dtype"));
+  if (!dtype_is_float(t)) fail(ASK_B200_E_UNSUPPORTED, "dtype must be f32, f16 or bf16");
+  return t;
+}
+
+// Weights, gates and tables: f32 or the activations' type.
+int parameter_type(const json::Value& r, const char* key, int activations) {
+  const json::Value* v = r.get(key);
+  const int t = v ? parse_dtype(v->as_str(key)) : int(kF32);
+  if (t != kF32 && t != activations) fail(ASK_B200_E_UNSUPPORTED, std::string(key) + " must be f32 or the step's dtype");
+  return t;
+}
+
+DropSite drop_site(const json::Value& r, const char* key) {
+  const double p = number_field(r, key, 0.0);
+  if (!(p >= 0.0 && p < 1.0)) fail(ASK_B200_E_INVALID, std::string(key) + " must be in [0, 1)");
+  const json::Value* id = r.get("stream_id");
+  const int64_t stream = id ? id->as_int("stream_id") : 0;
+  if (stream < 0 || stream > int64_t(UINT32_MAX)) fail(ASK_B200_E_INVALID, "stream_id must be in [0, 2^32)");
+  return DropSite{p > 0.0 ? 1u : 0u, uint32_t(std::floor(std::ldexp(p, 32))), uint32_t(stream), float(1.0 / (1.0 - p))};
+}
+
+// {"family": "dropout", "dtype", "count", "p", "stream_id", "residual"}: inputs
+// x, [residual], [seed i64[2] unless p is 0]; output y.
+void build_dropout(ask_b200_plan& pl, const json::Value& r) {
+  DropoutArgs& a = pl.drop;
+  a.type = activation_type(r);
+  a.count = checked_count(r.at("count"), "count");
+  a.drop = drop_site(r, "p");
+  const bool residual = bool_field(r, "residual", false);
+  pl.inputs.push_back({a.type, a.count, IM_FULL});
+  if (residual) pl.inputs.push_back({a.type, a.count, IM_FULL});
+  if (a.drop.on) pl.inputs.push_back({kI64, 2, IM_FULL});
+  pl.outputs = {{a.type, a.count, IM_FULL}};
+  pl.kernel = std::string(residual ? "dropout_residual_" : "dropout_") + kTypeNames[a.type];
+  pl.block = kDropThreads;
+  pl.launches = a.count ? 1 : 0;
+  int occ = blocks_per_sm_default(0);
+  if (pl.device >= 0) check_cuda(dropout_occupancy(a.type, residual, &occ), "occupancy");
+  if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
+  const uint64_t unit = a.type == kF32 ? 4 : 8;
+  const uint64_t needed = (a.count / unit + kDropThreads) / kDropThreads;
+  pl.grid = int(std::max<uint64_t>(1, std::min(needed, uint64_t(std::max(occ, 1)) * uint64_t(pl.num_sms))));
+}
+
+// How many chunks to cut each of `groups` equal stretches of `units` rows
+// into, one chunk a CTA, with `slots` CTAs running at once: the least time
+// (waves of CTAs x rows of a chunk), then the fewest chunks.
+uint64_t chunk_count(uint64_t groups, uint64_t units, uint64_t slots) {
+  const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(units, (2 * slots + groups - 1) / groups));
+  uint64_t best = 1, least = UINT64_MAX;
+  for (uint64_t c = 1; c <= most; ++c) {
+    const uint64_t time = ((groups * c + slots - 1) / slots) * ((units + c - 1) / c);
+    if (time < least) {
+      least = time;
+      best = c;
+    }
+  }
+  return best;
+}
+
+// {"family": "block_norm" | "block_norm_grad", "dtype", "rows", "cols", "norm":
+// "rms" | "layer", "eps", "branch", "post", "pre", "bias", "gate_groups",
+// "residual_scale", "dropout", "stream_id", "param_dtype"}.  Ports that a step's
+// switches leave out do not exist:
+//   block_norm       x, y, w_post, b_post, gate, w_pre, b_pre, seed ->
+//                    h, u, stats_post, stats_pre
+//   block_norm_grad  dh, du, h, y, w_post, b_post, gate, w_pre, stats_post, stats_pre, seed ->
+//                    dx, dy, dw_post, db_post, dgate, dw_pre, db_pre
+void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
+  NormArgs& a = pl.norm;
+  a.type = activation_type(r);
+  a.ptype = parameter_type(r, "param_dtype", a.type);
+  a.rows = checked_count(r.at("rows"), "rows");
+  const uint64_t cols = checked_count(r.at("cols"), "cols");
+  if (cols == 0) fail(ASK_B200_E_INVALID, "cols must be positive");
+  if (cols > uint64_t(kNormMaxCols))
+    fail(ASK_B200_E_UNSUPPORTED, "block norms take at most " + std::to_string(kNormMaxCols) + " columns");
+  a.cols = uint32_t(cols);
+  const std::string kind = r.get("norm") ? r.at("norm").as_str("norm") : "rms";
+  if (kind != "rms" && kind != "layer") fail(ASK_B200_E_INVALID, "norm must be 'rms' or 'layer'");
+  a.layer = kind == "layer";
+  a.branch = bool_field(r, "branch", true);
+  a.post = bool_field(r, "post", a.branch);
+  a.pre = bool_field(r, "pre", true);
+  a.bias = bool_field(r, "bias", false);
+  const json::Value* gg = r.get("gate_groups");
+  const uint64_t groups = gg ? checked_count(*gg, "gate_groups") : 0;
+  a.gated = groups > 0;
+  a.drop = drop_site(r, "dropout");
+  const double eps = number_field(r, "eps", 1e-6), alpha = number_field(r, "residual_scale", 1.0);
+  if (!(eps >= 0.0) || !std::isfinite(float(eps))) fail(ASK_B200_E_INVALID, "eps must be finite and not negative");
+  if (!std::isfinite(float(alpha))) fail(ASK_B200_E_INVALID, "residual_scale must be finite");
+  a.eps = float(eps);
+  a.alpha = float(alpha);
+  if (!a.branch && !a.pre) fail(ASK_B200_E_INVALID, "a step without a branch needs its pre norm");
+  if (!a.branch && (a.post || a.gated || a.drop.on || a.alpha != 1.0f))
+    fail(ASK_B200_E_INVALID, "post norm, gate, dropout and residual scale belong to a branch");
+  if (a.bias && !a.post && !a.pre) fail(ASK_B200_E_INVALID, "bias belongs to a norm");
+  if (a.gated && (groups > UINT32_MAX || a.rows % groups))
+    fail(ASK_B200_E_INVALID, "gate_groups must divide rows");
+  a.groups = a.gated ? uint32_t(groups) : 1;
+  a.rows_per_group = a.rows / a.groups;
+
+  const uint64_t n = mul_checked(a.rows, cols), gate = mul_checked(groups, cols), width = a.layer ? 2 : 1;
+  auto in = [&](bool on, int type, uint64_t elements) { if (on) pl.inputs.push_back({type, elements, IM_FULL}); };
+  auto out = [&](bool on, int type, uint64_t elements) { if (on) pl.outputs.push_back({type, elements, IM_FULL}); };
+  const bool post_bias = a.post && a.bias, pre_bias = a.pre && a.bias, need_y = a.post || a.gated;
+  if (!grad) {
+    in(true, a.type, n);
+    in(a.branch, a.type, n);
+    in(a.post, a.ptype, cols);
+    in(post_bias, a.ptype, cols);
+    in(a.gated, a.ptype, gate);
+    in(a.pre, a.ptype, cols);
+    in(pre_bias, a.ptype, cols);
+    out(a.branch, a.type, n);
+    out(a.pre, a.type, n);
+    out(a.post, kF32, a.rows * width);
+    out(a.pre, kF32, a.rows * width);
+  } else {
+    in(a.branch, a.type, n);
+    in(a.pre, a.type, n);
+    in(a.pre, a.type, n);
+    in(need_y, a.type, n);
+    in(a.post, a.ptype, cols);
+    in(post_bias && a.gated, a.ptype, cols);
+    in(a.gated, a.ptype, gate);
+    in(a.pre, a.ptype, cols);
+    in(a.post, kF32, a.rows * width);
+    in(a.pre, kF32, a.rows * width);
+    out(true, a.type, n);
+    out(a.branch, a.type, n);
+    out(a.post, kF32, cols);
+    out(post_bias, kF32, cols);
+    out(a.gated, kF32, gate);
+    out(a.pre, kF32, cols);
+    out(pre_bias, kF32, cols);
+  }
+  in(a.drop.on, kI64, 2);
+
+  a.shape = norm_shape(cols, grad);
+  pl.block = a.shape.threads;
+  int occ = 2;
+  if (pl.device >= 0) check_cuda(norm_occupancy(a, grad, &occ), "occupancy");
+  if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
+  const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
+  const uint64_t teams = a.shape.warp_teams ? uint64_t(a.shape.threads) / 32 : 1;
+  const std::string name = std::string(a.layer ? "layer_" : "rms_") + kTypeNames[a.type];
+  if (!grad) {
+    pl.kernel = "norm_rows_" + name;
+    pl.grid = int(std::max<uint64_t>(1, std::min<uint64_t>((a.rows + teams - 1) / teams, slots)) * uint64_t(a.shape.ctas));
+    pl.launches = a.rows ? 1 : 0;
+    return;
+  }
+  pl.kernel = "norm_grad_" + name;
+  a.chunks = uint32_t(chunk_count(a.groups, (a.rows_per_group + teams - 1) / teams, slots));
+  const uint64_t places = mul_checked(a.groups, a.chunks);
+  if (places * uint64_t(a.shape.ctas) > uint64_t(INT32_MAX)) fail(ASK_B200_E_UNSUPPORTED, "too many gate groups");
+  pl.grid = int(places * uint64_t(a.shape.ctas));
+  const int kinds = norm_sums(a).count();
+  pl.scratch = size_t(mul_checked(mul_checked(places, cols), uint64_t(kinds) * sizeof(float)));
+  pl.launches = (a.rows ? 1 : 0) + (kinds ? 1 : 0);
+}
+
+// {"family": "bias_softmax" | "bias_softmax_grad", "dtype", "batch", "heads",
+// "queries", "keys", "thresholds": [...], "bidirectional", "scale", "causal",
+// "lengths", "offsets", "dropout", "stream_id", "table_dtype"}:
+//   bias_softmax       s, table, [lengths], [offsets], [seed] -> p, lse
+//   bias_softmax_grad  s, dp, lse, table, [lengths], [offsets], [seed] -> ds, dtable
+void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
+  BiasSoftmaxArgs& a = pl.bias;
+  a.type = activation_type(r);
+  a.table_type = parameter_type(r, "table_dtype", a.type);
+  a.batch = checked_count(r.at("batch"), "batch");
+  const uint64_t heads = checked_count(r.at("heads"), "heads"), keys = checked_count(r.at("keys"), "keys");
+  a.queries = checked_count(r.at("queries"), "queries");
+  if (heads > (1u << 20)) fail(ASK_B200_E_UNSUPPORTED, "at most 2^20 heads");
+  if (a.queries > (uint64_t(1) << 30)) fail(ASK_B200_E_UNSUPPORTED, "at most 2^30 queries");
+  if (keys > kBiasMaxKeys) fail(ASK_B200_E_UNSUPPORTED, "at most " + std::to_string(kBiasMaxKeys) + " keys");
+  a.heads = uint32_t(heads);
+  a.keys = uint32_t(keys);
+  const auto& th = r.at("thresholds").as_array("thresholds");
+  if (th.empty() || th.size() > size_t(kBiasMaxThresholds))
+    fail(ASK_B200_E_UNSUPPORTED, "1.." + std::to_string(kBiasMaxThresholds) + " bucket thresholds");
+  int64_t last = 0;
+  for (const json::Value& v : th) {
+    const int64_t t = v.as_int("threshold");
+    // equal ones skip a bucket, as geometric steps of less than one distance do
+    if (t < 1 || t < last) fail(ASK_B200_E_INVALID, "bucket thresholds must be positive and must not fall");
+    if (t > kBiasMaxDistance)
+      fail(ASK_B200_E_UNSUPPORTED, "bucket thresholds must be at most " + std::to_string(kBiasMaxDistance));
+    a.thresholds[a.n_thresholds++] = int(t);
+    last = t;
+  }
+  a.bidirectional = bool_field(r, "bidirectional", true);
+  a.buckets = uint32_t((a.n_thresholds + 1) * (a.bidirectional ? 2 : 1));
+  const double scale = number_field(r, "scale", 1.0);
+  if (!std::isfinite(float(scale))) fail(ASK_B200_E_INVALID, "scale must be finite");
+  a.scale = float(scale);
+  a.causal = bool_field(r, "causal", false);
+  a.drop = drop_site(r, "dropout");
+  const bool lengths = bool_field(r, "lengths", false), offsets = bool_field(r, "offsets", false);
+
+  const uint64_t rows = mul_checked(mul_checked(a.batch, heads), a.queries), n = mul_checked(rows, keys);
+  const uint64_t table = mul_checked(a.buckets, heads);
+  pl.inputs.push_back({a.type, n, IM_FULL});
+  if (grad) {
+    pl.inputs.push_back({a.type, n, IM_FULL});
+    pl.inputs.push_back({kF32, rows, IM_FULL});
+  }
+  pl.inputs.push_back({a.table_type, table, IM_FULL});
+  if (lengths) pl.inputs.push_back({kI32, a.batch, IM_FULL});
+  if (offsets) pl.inputs.push_back({kI32, a.batch, IM_FULL});
+  if (a.drop.on) pl.inputs.push_back({kI64, 2, IM_FULL});
+  if (grad) pl.outputs = {{a.type, n, IM_FULL}, {kF32, table, IM_FULL}};
+  else pl.outputs = {{a.type, n, IM_FULL}, {kF32, rows, IM_FULL}};
+  // presence, until a launch puts the addresses here
+  a.lengths = lengths ? reinterpret_cast<const int*>(1) : nullptr;
+  a.offsets = offsets ? reinterpret_cast<const int*>(1) : nullptr;
+
+  a.shape = bias_softmax_shape(keys, rows, a.type, grad, pl.num_sms);
+  if (a.shape.threads * a.shape.elems > kBiasMaxRowPerCta)
+    fail(ASK_B200_E_UNSUPPORTED, "rows that start inside a 16-byte unit take at most " +
+                                     std::to_string(kBiasMaxKeys - 7) + " keys");
+  bias_softmax_shared(&a, grad);
+  pl.block = a.shape.threads;
+  int occ = 2;
+  if (pl.device >= 0) check_cuda(bias_softmax_occupancy(a, grad, &occ), "occupancy");
+  if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
+  const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
+  const uint64_t teams = a.shape.warp_teams ? uint64_t(a.shape.threads) / 32 : 1;
+  const uint64_t pairs = mul_checked(a.batch, a.queries);
+  a.chunks = heads ? uint32_t(chunk_count(heads, (pairs + teams - 1) / teams, slots)) : 1;
+  const uint64_t ctas = mul_checked(mul_checked(heads, a.chunks), uint64_t(a.shape.ctas));
+  if (ctas > uint64_t(INT32_MAX)) fail(ASK_B200_E_UNSUPPORTED, "too many heads");
+  pl.grid = int(std::max<uint64_t>(1, ctas));
+  pl.kernel = std::string(grad ? "bias_softmax_grad_" : "bias_softmax_") + kTypeNames[a.type];
+  pl.launches = (rows ? 1 : 0) + (grad && table ? 1 : 0);
+  if (grad && rows) pl.scratch = size_t(ctas * a.buckets * sizeof(float));
+}
+
 // The diagnostics the reference's CUDA lowering reports for a step
 // (lib/Lowering/CUDA.cpp:408-417, "cuda_lowering"), for the kernels this plan
 // launches: the same fields with the same meaning, plus the plan's strategy.
@@ -858,7 +1121,7 @@ void build_softmax(ask_b200_plan& pl, const json::Value& r) {
 // reduction of a step folds in the same pass); input_load_count counts input
 // ports, each read once per element.  pre_copy names the step's base input.
 std::string cuda_lowering(const ask_b200_plan& pl, long pre_copy_input) {
-  const bool reduce = pl.family == FAM_REDUCE, softmax = pl.family == FAM_SOFTMAX;
+  const bool reduce = pl.family == FAM_REDUCE, softmax = row_family(pl.family);
   const bool warp = (reduce && !pl.views && pl.strategy == RS_WARP_ROW) || softmax;
   const int block = pl.sm_step ? pl.block : pl.family == FAM_ELEMENTWISE ? kEwThreads : reduce ? kRedThreads
                   : softmax ? pl.block : 256;
@@ -870,7 +1133,7 @@ std::string cuda_lowering(const ask_b200_plan& pl, long pre_copy_input) {
   }
   uint64_t count = pl.outputs.empty() ? 0 : pl.outputs[0].elements;
   if (pl.family == FAM_SCATTER && pl.inputs.size() > 2) count = pl.inputs[2].elements;
-  if (softmax) count = pl.sm.rows;
+  if (pl.family == FAM_SOFTMAX) count = pl.sm.rows;
   uint64_t per_output = warp ? (softmax || pl.sm_step ? uint64_t(pl.block) : 32) : 1;
   if (reduce && !pl.views && pl.strategy == RS_SPLIT) per_output = uint64_t(pl.grid) * uint64_t(block);
   const char* strat[] = {"warp_row", "column", "split"};
@@ -898,7 +1161,7 @@ std::string describe(const ask_b200_plan& pl) {
     << kFamilyNames[pl.family] << "\",\"kernel\":\"" << pl.kernel << "\",\"device\":" << pl.device
     << ",\"target\":{\"backend\":\"cuda\",\"arch\":100},\"launch\":{\"grid\":[" << pl.grid << "," << pl.col_chunks << ",1],\"block\":["
     << (pl.sm_step ? pl.block : pl.family == FAM_ELEMENTWISE ? kEwThreads : pl.family == FAM_REDUCE ? kRedThreads :
-        pl.family == FAM_SOFTMAX ? pl.block : 256)
+        row_family(pl.family) ? pl.block : 256)
     << ",1,1],\"shared_bytes\":0},\"kernels_per_launch\":" << pl.launches << ",\"scratch_bytes\":" << pl.scratch;
   if (pl.family == FAM_REDUCE) {
     const char* strat[] = {"warp_row", "column", "split"};
@@ -923,7 +1186,7 @@ std::string describe(const ask_b200_plan& pl) {
   // (lib/Lowering/CUDA.cpp:392-407): arguments are the ports in port order.
   const int block = pl.sm_step ? pl.block : pl.family == FAM_ELEMENTWISE ? kEwThreads
                     : pl.family == FAM_REDUCE ? kRedThreads
-                    : pl.family == FAM_SOFTMAX ? pl.block : 256;
+                    : row_family(pl.family) ? pl.block : 256;
   o << "],\"invocation\":{\"version\":2,\"kind\":\"ask-b200-recipe\",\"grid\":[" << pl.grid
     << ",1,1],\"block\":[" << block << ",1,1],\"shared_bytes\":0,\"arguments\":[";
   for (size_t k = 0; k < pl.inputs.size() + pl.outputs.size(); ++k)
@@ -1085,6 +1348,101 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
       if (a.rows && (!aligned16(ports[0]) || !aligned16(ports[3])))
         fail(ASK_B200_E_INVALID, "the fused softmax needs 16-byte aligned x and y");
       check_cuda(softmax_rows_launch(a, pl.num_sms, st), "softmax launch");
+      break;
+    }
+    case FAM_DROPOUT: {
+      DropoutArgs a = pl.drop;
+      const uint64_t* at = ports;
+      a.x = reinterpret_cast<const void*>(*at++);
+      if (ni > size_t(a.drop.on ? 2 : 1)) a.residual = reinterpret_cast<const void*>(*at++);
+      if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
+      a.y = reinterpret_cast<void*>(*at);
+      check_cuda(dropout_launch(a, pl.grid, st), "dropout launch");
+      break;
+    }
+    case FAM_BLOCK_NORM:
+    case FAM_BLOCK_NORM_GRAD: {
+      NormArgs a = pl.norm;
+      const uint64_t* at = ports;
+      const uint64_t vec = a.type == kF32 ? 4 : 8;
+      bool wide = a.cols % vec == 0;
+      auto in = [&](bool on, const void*& p, bool row = true) {
+        if (!on) return;
+        if (row) wide &= aligned16(*at);
+        p = reinterpret_cast<const void*>(*at++);
+      };
+      auto stats = [&](bool on, const float*& p) { if (on) p = reinterpret_cast<const float*>(*at++); };
+      auto out = [&](bool on, void*& p) {
+        if (!on) return;
+        wide &= aligned16(*at);
+        p = reinterpret_cast<void*>(*at++);
+      };
+      auto out32 = [&](bool on, float*& p) { if (on) p = reinterpret_cast<float*>(*at++); };
+      const bool post_bias = a.post && a.bias, pre_bias = a.pre && a.bias;
+      if (pl.family == FAM_BLOCK_NORM) {
+        in(true, a.x);
+        in(a.branch, a.y);
+        in(a.post, a.w_post);
+        in(post_bias, a.b_post);
+        in(a.gated, a.gate);
+        in(a.pre, a.w_pre);
+        in(pre_bias, a.b_pre);
+        if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
+        out(a.branch, a.h);
+        out(a.pre, a.u);
+        out32(a.post, a.stats_post);
+        out32(a.pre, a.stats_pre);
+        check_cuda(norm_launch(a, wide, pl.grid, st), "block_norm launch");
+        break;
+      }
+      in(a.branch, a.dh);
+      in(a.pre, a.du);
+      in(a.pre, a.h_in);
+      in(a.post || a.gated, a.y);
+      in(a.post, a.w_post);
+      in(post_bias && a.gated, a.b_post);
+      in(a.gated, a.gate);
+      in(a.pre, a.w_pre);
+      stats(a.post, a.stats_post_in);
+      stats(a.pre, a.stats_pre_in);
+      if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
+      out(true, a.dx);
+      out(a.branch, a.dy);
+      out32(a.post, a.dw_post);
+      out32(post_bias, a.db_post);
+      out32(a.gated, a.dgate);
+      out32(a.pre, a.dw_pre);
+      out32(pre_bias, a.db_pre);
+      if (pl.scratch && !scratch) fail(ASK_B200_E_INVALID, "this plan needs scratch memory");
+      if (scratch && !aligned16(scratch)) fail(ASK_B200_E_INVALID, "scratch must be 16-byte aligned");
+      a.partial = reinterpret_cast<float*>(scratch);
+      check_cuda(norm_grad_launch(a, wide, st), "block_norm_grad launch");
+      break;
+    }
+    case FAM_BIAS_SOFTMAX:
+    case FAM_BIAS_SOFTMAX_GRAD: {
+      BiasSoftmaxArgs a = pl.bias;
+      const bool grad = pl.family == FAM_BIAS_SOFTMAX_GRAD;
+      const uint64_t* at = ports;
+      a.aligned = aligned16(*at);
+      a.s = reinterpret_cast<const void*>(*at++);
+      if (grad) {
+        a.aligned = a.aligned && aligned16(*at);
+        a.dp = reinterpret_cast<const void*>(*at++);
+        a.lse_in = reinterpret_cast<const float*>(*at++);
+      }
+      a.table = reinterpret_cast<const void*>(*at++);
+      if (a.lengths) a.lengths = reinterpret_cast<const int*>(*at++);
+      if (a.offsets) a.offsets = reinterpret_cast<const int*>(*at++);
+      if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
+      a.aligned = a.aligned && aligned16(*at);
+      a.out = reinterpret_cast<void*>(*at++);
+      if (grad) a.dtable = reinterpret_cast<float*>(*at);
+      else a.lse = reinterpret_cast<float*>(*at);
+      if (pl.scratch && !scratch) fail(ASK_B200_E_INVALID, "this plan needs scratch memory");
+      if (scratch && !aligned16(scratch)) fail(ASK_B200_E_INVALID, "scratch must be 16-byte aligned");
+      a.partial = reinterpret_cast<float*>(scratch);
+      check_cuda(bias_softmax_launch(a, grad, st), "bias_softmax launch");
       break;
     }
     default:
@@ -1327,6 +1685,11 @@ int ask_b200_plan_create(const char* recipe_json, int device, ask_b200_plan** ou
     else if (fam == "gather") { pl->family = FAM_GATHER; build_index(*pl, r, false); }
     else if (fam == "scatter_add") { pl->family = FAM_SCATTER; build_index(*pl, r, true); }
     else if (fam == "softmax") { pl->family = FAM_SOFTMAX; build_softmax(*pl, r); }
+    else if (fam == "dropout") { pl->family = FAM_DROPOUT; build_dropout(*pl, r); }
+    else if (fam == "block_norm") { pl->family = FAM_BLOCK_NORM; build_norm(*pl, r, false); }
+    else if (fam == "block_norm_grad") { pl->family = FAM_BLOCK_NORM_GRAD; build_norm(*pl, r, true); }
+    else if (fam == "bias_softmax") { pl->family = FAM_BIAS_SOFTMAX; build_bias_softmax(*pl, r, false); }
+    else if (fam == "bias_softmax_grad") { pl->family = FAM_BIAS_SOFTMAX_GRAD; build_bias_softmax(*pl, r, true); }
     else fail(ASK_B200_E_UNSUPPORTED, "unknown family '" + fam + "'");
     if (pl->inputs.size() + pl->outputs.size() > 64)
       fail(ASK_B200_E_UNSUPPORTED, "the pointer ABI supports at most 64 input and output buffers");

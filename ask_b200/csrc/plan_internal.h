@@ -10,7 +10,8 @@
 
 namespace askb {
 
-enum Family { FAM_ELEMENTWISE = 0, FAM_REDUCE, FAM_GATHER, FAM_SCATTER, FAM_SOFTMAX };
+enum Family { FAM_ELEMENTWISE = 0, FAM_REDUCE, FAM_GATHER, FAM_SCATTER, FAM_SOFTMAX,
+              FAM_DROPOUT, FAM_BLOCK_NORM, FAM_BLOCK_NORM_GRAD, FAM_BIAS_SOFTMAX, FAM_BIAS_SOFTMAX_GRAD };
 
 struct PortInfo {
   int dtype;
@@ -37,6 +38,9 @@ struct ask_b200_plan {
   askb::RedArgs red{};
   askb::IndexArgs idx{};
   askb::SoftmaxArgs sm{};
+  askb::DropoutArgs drop{};
+  askb::NormArgs norm{};
+  askb::BiasSoftmaxArgs bias{};
   bool views = false;  // elementwise step with IM_VIEW ports or coordinate instructions
   askb::ViewSet vs{};
   bool shardable = false;

@@ -1,0 +1,163 @@
+// The threads that share a row, and their reductions.
+//
+// A row is held by a warp (short rows: several independent teams in a CTA, no
+// barrier), by a CTA, or by a cluster of up to eight CTAs (rows longer than a
+// CTA's registers hold, or so few rows that most SMs would idle).  A reduction
+// folds each warp by shuffles, then every warp writes its record into the
+// shared memory of every CTA of the team (distributed shared memory within a
+// cluster), one barrier follows, and every thread folds the records in warp
+// order: one barrier a reduction whatever the team, and every thread gets the
+// same bits.
+//
+// Records are kept in two sets by the row's parity: a thread writes a row's
+// records only after the barrier of the row before, which no thread passes
+// until all have read the records of the row before that.  Reductions of one
+// row use slots of their own.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace askb {
+
+constexpr int kTeamThreads = 512;                   // threads of a CTA at most
+constexpr int kTeamCluster = 8;                     // CTAs of a team at most (the portable cluster size)
+constexpr int kTeamRecords = kTeamThreads / 32 * kTeamCluster;
+
+struct Team {
+  uint32_t tid;      // thread within this CTA's part of the team
+  uint32_t threads;  // threads of that part
+  uint32_t lane, warp, warps;
+  uint32_t ctas, rank;  // CTAs of the team (the cluster) and this one's place among them
+};
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(const void* mine, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+  return r;
+}
+
+// `warp_teams`: every warp is a team of its own.
+__device__ __forceinline__ Team team_of(bool warp_teams) {
+  Team t;
+  t.lane = threadIdx.x & 31u;
+  if (warp_teams) {
+    t.tid = t.lane;
+    t.threads = 32;
+    t.warp = 0;
+    t.warps = 1;
+    t.ctas = 1;
+    t.rank = 0;
+  } else {
+    t.tid = threadIdx.x;
+    t.threads = blockDim.x;
+    t.warp = threadIdx.x >> 5;
+    t.warps = blockDim.x >> 5;
+    t.ctas = cluster_size();
+    t.rank = cluster_rank();
+  }
+  return t;
+}
+
+// Before the first reduction: a CTA's shared memory may be written by a peer
+// only once that CTA runs.
+__device__ __forceinline__ void team_start(const Team& t) {
+  if (t.ctas > 1) cluster_barrier();
+}
+
+template <int N>
+struct TeamRecords {
+  float v[2][kTeamRecords][N];
+};
+
+// Write this warp's record (v, the same in all lanes) to the team; then barrier.
+template <int N>
+__device__ __forceinline__ void team_exchange(const Team& t, TeamRecords<N>& sh, int parity, const float (&v)[N]) {
+  if (t.ctas == 1) {
+    if (t.lane == 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) sh.v[parity][t.warp][n] = v[n];
+    }
+    __syncthreads();
+    return;
+  }
+  if (t.lane < t.ctas) {
+    const uint32_t at = peer_address(&sh.v[parity][t.rank * t.warps + t.warp][0], t.lane);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4u * n), "f"(v[n]) : "memory");
+  }
+  cluster_barrier();
+}
+
+// Sum of N values over the team, the same bits in every thread.
+template <int N>
+__device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int parity, float (&v)[N]) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], d);
+  }
+  const uint32_t records = t.warps * t.ctas;
+  if (records == 1) return;
+  team_exchange<N>(t, sh, parity, v);
+  if (records <= 8) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = sh.v[parity][0][n];
+    for (uint32_t k = 1; k < records; ++k) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += sh.v[parity][k][n];
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = 0.0f;
+      for (uint32_t k = t.lane; k < records; k += 32) v[n] += sh.v[parity][k][n];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], d);
+    }
+  }
+}
+
+// Launch of a row kernel: CTAs of the shape's threads in clusters of its size,
+// as a programmatic dependent (pdl.cuh).
+inline cudaError_t launch_rows(const void* kernel, const TeamShape& s, unsigned grid, unsigned shared_bytes, void** args,
+                               cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(unsigned(s.threads));
+  cfg.dynamicSmemBytes = shared_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(s.ctas);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s.ctas > 1 ? 2 : 1;
+  (void)cudaLaunchKernelExC(&cfg, kernel, args);
+  return cudaGetLastError();
+}
+
+}  // namespace askb

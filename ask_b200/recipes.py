@@ -112,6 +112,107 @@ def scatter_add(dtype: str, index_dtype: str, dim: int, inner: int, n: int, oute
             "dim": int(dim), "inner": int(inner), "n": int(n), "pre_copy": {"input": 0, "output": 0}}
 
 
+# ---- training-block operators ---------------------------------------------------------
+# Row work between a transformer's matrix products.  Ports that a step's switches
+# leave out do not exist; the others keep the order given with each builder.  The
+# seed port is i64[2] {seed, offset} on the device: element i of a step draws word
+# i % 4 of the Philox4x32-10 block offset + i / 4 (see csrc/philox.cuh), so the
+# gradient step takes the same seed, and a training step advances the offset by
+# (elements + 3) // 4.  `stream_id` keeps the sites of one model apart.
+def dropout(dtype: str, count: int, p: float, stream_id: int = 0, residual: bool = False) -> dict:
+    """y = dropout(x) (+ residual): x, [residual], [seed] -> y.  The gradient of
+    the dropped part is the same step, without the residual, applied to dy."""
+    return {"family": "dropout", "dtype": dtype, "count": int(count), "p": float(p), "stream_id": int(stream_id),
+            "residual": bool(residual)}
+
+
+def block_norm(dtype: str, rows: int, cols: int, norm: str = "rms", eps: float = 1e-6, branch: bool = True,
+               post: bool | None = None, pre: bool = True, bias: bool = False, gate_groups: int = 0,
+               residual_scale: float = 1.0, dropout: float = 0.0, stream_id: int = 0, param_dtype: str = "f32") -> dict:
+    """h = residual_scale * x + D(gate * N_post(y)), u = N_pre(h):
+    x, [y], [w_post], [b_post], [gate], [w_pre], [b_pre], [seed] ->
+    [h], [u], [stats_post], [stats_pre].
+
+    ``branch=False`` leaves u = N_pre(x) alone; ``post``/``pre`` drop a norm; gate
+    is [gate_groups, cols], one for each of that many equal runs of rows (1: per
+    channel, rows: per token).  stats are what the gradient needs of each row:
+    1 / sqrt(var + eps), after the mean for a layer norm."""
+    return _norm("block_norm", dtype, rows, cols, norm, eps, branch, post, pre, bias, gate_groups, residual_scale,
+                 dropout, stream_id, param_dtype)
+
+
+def block_norm_grad(dtype: str, rows: int, cols: int, norm: str = "rms", eps: float = 1e-6, branch: bool = True,
+                    post: bool | None = None, pre: bool = True, bias: bool = False, gate_groups: int = 0,
+                    residual_scale: float = 1.0, dropout: float = 0.0, stream_id: int = 0,
+                    param_dtype: str = "f32") -> dict:
+    """Gradient of :func:`block_norm` from dh and du, the gradients to h and u:
+    [dh], [du], [h], [y], [w_post], [b_post], [gate], [w_pre], [stats_post], [stats_pre], [seed] ->
+    dx, [dy], [dw_post], [db_post], [dgate], [dw_pre], [db_pre]
+    (y with a post norm or a gate, b_post with a gate; parameter gradients are f32)."""
+    return _norm("block_norm_grad", dtype, rows, cols, norm, eps, branch, post, pre, bias, gate_groups, residual_scale,
+                 dropout, stream_id, param_dtype)
+
+
+def _norm(family, dtype, rows, cols, norm, eps, branch, post, pre, bias, gate_groups, residual_scale, dropout,
+          stream_id, param_dtype) -> dict:
+    return {"family": family, "dtype": dtype, "rows": int(rows), "cols": int(cols), "norm": norm, "eps": float(eps),
+            "branch": bool(branch), "post": bool(branch if post is None else post), "pre": bool(pre),
+            "bias": bool(bias), "gate_groups": int(gate_groups), "residual_scale": float(residual_scale),
+            "dropout": float(dropout), "stream_id": int(stream_id), "param_dtype": param_dtype}
+
+
+def bucket_thresholds(num_buckets: int, max_distance: int, bidirectional: bool = True) -> list:
+    """Distances at which the bucket of a relative position grows by one: single
+    distances for half of a side's buckets, then steps growing geometrically to
+    ``max_distance``; found with whole numbers, so no distance falls into a
+    neighbouring bucket by rounding."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    single = side // 2
+    if single < 1 or (bidirectional and num_buckets % 2) or max_distance <= single:
+        raise ValueError("bucket_thresholds needs 2 buckets a side or more and a max_distance beyond half of them")
+    steps = side - single
+    thresholds, n = list(range(1, single + 1)), single
+    for j in range(1, steps):  # the least n with (n / single)^steps >= (max_distance / single)^j
+        while n ** steps * single ** j < max_distance ** j * single ** steps:
+            n += 1
+        thresholds.append(n)
+    return thresholds
+
+
+def bias_softmax(dtype: str, batch: int, heads: int, queries: int, keys: int, thresholds: list,
+                 bidirectional: bool = True, scale: float = 1.0, causal: bool = False, lengths: bool = False,
+                 offsets: bool = False, dropout: float = 0.0, stream_id: int = 0, table_dtype: str = "f32") -> dict:
+    """p = D(softmax(scale * s + table[bucket(k - q - offset), head])) over the keys
+    that the lengths and the causal rule leave, and lse, the log of the sum:
+    s [batch, heads, queries, keys], table [buckets, heads], [lengths i32[batch]],
+    [offsets i32[batch]], [seed] -> p, lse [batch, heads, queries] f32.
+
+    Buckets count the thresholds at or below the distance (``bidirectional``: twice
+    len(thresholds) + 1 of them, the second half for keys after the query).  A row
+    without keys gives zeros and lse = -inf.  Single tokens: queries = 1, offsets =
+    the token's position."""
+    return _bias_softmax("bias_softmax", dtype, batch, heads, queries, keys, thresholds, bidirectional, scale, causal,
+                         lengths, offsets, dropout, stream_id, table_dtype)
+
+
+def bias_softmax_grad(dtype: str, batch: int, heads: int, queries: int, keys: int, thresholds: list,
+                      bidirectional: bool = True, scale: float = 1.0, causal: bool = False, lengths: bool = False,
+                      offsets: bool = False, dropout: float = 0.0, stream_id: int = 0,
+                      table_dtype: str = "f32") -> dict:
+    """Gradient of :func:`bias_softmax`: s, dp, lse, table, [lengths], [offsets],
+    [seed] -> ds, dtable [buckets, heads] f32."""
+    return _bias_softmax("bias_softmax_grad", dtype, batch, heads, queries, keys, thresholds, bidirectional, scale,
+                         causal, lengths, offsets, dropout, stream_id, table_dtype)
+
+
+def _bias_softmax(family, dtype, batch, heads, queries, keys, thresholds, bidirectional, scale, causal, lengths,
+                  offsets, dropout, stream_id, table_dtype) -> dict:
+    return {"family": family, "dtype": dtype, "batch": int(batch), "heads": int(heads), "queries": int(queries),
+            "keys": int(keys), "thresholds": [int(t) for t in thresholds], "bidirectional": bool(bidirectional),
+            "scale": float(scale), "causal": bool(causal), "lengths": bool(lengths), "offsets": bool(offsets),
+            "dropout": float(dropout), "stream_id": int(stream_id), "table_dtype": table_dtype}
+
+
 # ---- the benchmark configurations ---------------------------------------------------
 def cfg1_step(count: int = 4096 * 4096) -> dict:
     p = Program()

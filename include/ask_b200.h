@@ -66,6 +66,10 @@ ASK_B200_API const char *ask_b200_last_error(void);
  * (lib/Lowering/CUDA.cpp:152) plus Session::load (lib/Runtime/CUDA.cpp:499-546)
  * for owned steps: the recipe names the step's family (elementwise, reduce,
  * gather, scatter_add), port types and static sizes, and its op program.
+ * Five families beyond ASK's owned steps are the row work of a transformer
+ * block between its matrix products: dropout, block_norm, block_norm_grad,
+ * bias_softmax and bias_softmax_grad (ask_b200/recipes.py has their fields and
+ * ports).  They launch, report errors and take scratch like the others.
  * device = -1 builds a host-only plan (validation and describe only; launching
  * it fails), which needs no GPU.
  */

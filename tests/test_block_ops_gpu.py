@@ -1,0 +1,544 @@
+"""Training-block operators on the GPU, through the C ABI, against plain 64-bit forms (block_ops_ref.py, which also
+derives the tolerances)."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ask_b200
+import block_ops_ref as ref
+from ask_b200 import recipes as R
+
+pytestmark = pytest.mark.gpu
+TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i32": torch.int32, "i64": torch.int64}
+
+
+def dev(a, dtype, skew=0):
+    """A device tensor that starts `skew` elements into a 16-byte aligned allocation."""
+    t = torch.as_tensor(np.ascontiguousarray(a)) if not torch.is_tensor(a) else a
+    buf = torch.empty(t.numel() + skew + 16, dtype=TORCH[dtype], device="cuda")
+    buf[skew:skew + t.numel()].copy_(t.reshape(-1).to(TORCH[dtype]))
+    return buf[skew:skew + t.numel()]
+
+
+def rounded(rng, shape, dtype, mean=0.0, std=1.0):
+    """Values of the stored type, as f64."""
+    v = torch.from_numpy(rng.standard_normal(shape) * std + mean).to(TORCH[dtype])
+    return v.double().numpy()
+
+
+def host(t, shape):
+    return t.double().cpu().numpy().reshape(shape)
+
+
+def launch(recipe, inputs, skew=0, stream=None):
+    """Outputs of one launch; 16 guard elements behind each stay as they were."""
+    plan = ask_b200.Plan(recipe, device=0)
+    pm = plan.describe()["port_map"]
+    assert [p["elements"] for p in pm[:plan.n_inputs]] == [t.numel() for t in inputs]
+    outs, whole = [], []
+    for p in pm[plan.n_inputs:]:
+        s = skew if p["element_type"] != "f32" or recipe["dtype"] == "f32" else 0
+        buf = torch.full((p["elements"] + s + 16,), 77, dtype=TORCH[p["element_type"]], device="cuda")
+        whole.append((buf, s, p["elements"]))
+        outs.append(buf[s:s + p["elements"]])
+    scratch = torch.full((plan.scratch_bytes,), 0xA5, dtype=torch.uint8, device="cuda") if plan.scratch_bytes else None
+    plan.launch(inputs, outs, scratch, stream or torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    for buf, s, n in whole:
+        assert bool((buf[:s] == 77).all()) and bool((buf[s + n:] == 77).all()), "written outside an output"
+    return outs
+
+
+def close(got, value, tol, what):
+    bad = ~((np.abs(got - value) <= tol) | (got == value) | (np.isnan(got) & np.isnan(value)))
+    assert not bad.any(), "%s: %d of %d off, worst %.3g of its tolerance" % (
+        what, bad.sum(), bad.size, np.nanmax(np.abs(got - value)[bad] / np.broadcast_to(tol, bad.shape)[bad]))
+
+
+# ---- dropout -------------------------------------------------------------------------------
+def dropout_exact(x, r, p, seed, offset, stream, dtype):
+    """Bit for bit: one 32-bit product by 1 / (1 - p), one 32-bit sum, one rounding."""
+    keep = ref.keep_mask(p, seed, offset, stream, x.shape)
+    y = np.where(keep, x.astype(np.float32) * np.float32(1.0 / (1.0 - p)), np.float32(0))
+    if r is not None:
+        y = y + r.astype(np.float32)
+    return torch.from_numpy(y.astype(np.float32)).to(TORCH[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("count", [1, 3, 4, 8, 9, 1000, 4099, 300_001])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("skew", [0, 1])
+def test_dropout(device, dtype, count, residual, skew):
+    rng = np.random.default_rng(count)
+    x = rounded(rng, count, dtype, std=3.0)
+    r = rounded(rng, count, dtype) if residual else None
+    seed, offset, stream, p = -12345678901234, 2 ** 32 - 5, 9, 0.3
+    ins = [dev(x, dtype, skew)] + ([dev(r, dtype, skew)] if residual else []) + [dev(np.array([seed, offset]), "i64")]
+    y, = launch(R.dropout(dtype, count, p, stream_id=stream, residual=residual), ins, skew)
+    assert torch.equal(y.cpu(), dropout_exact(x, r, p, seed, offset, stream, dtype))
+
+
+def test_dropout_edges(device):
+    n = 5000
+    seed = dev(np.array([1, 2]), "i64")
+    x = np.full(n, np.nan)
+    x[::2] = np.inf
+    y, = launch(R.dropout("f32", n, 0.5), [dev(x, "f32"), seed])
+    keep = ref.keep_mask(0.5, 1, 2, 0, (n,))
+    got = host(y, n)
+    assert (got[~keep] == 0).all() and np.isnan(got[keep & np.isnan(x)]).all() and np.isinf(got[keep & np.isinf(x)]).all()
+    # p = 0 copies and reads no seed; the offset wraps at 2^64
+    z, = launch(R.dropout("bf16", n, 0.0), [dev(np.arange(n) % 250, "bf16")])
+    assert (host(z, n) == np.arange(n) % 250).all()
+    ones = np.ones(n)
+    y, = launch(R.dropout("f32", n, 0.25), [dev(ones, "f32"), dev(np.array([3, -7]), "i64")])
+    assert torch.equal(y.cpu(), dropout_exact(ones, None, 0.25, 3, -7, 0, "f32"))
+
+
+def test_dropout_rate_and_sites(device):
+    """The share kept is that of n independent draws, within six deviations; sites and seeds are unlike."""
+    n, p = 1 << 20, 0.1
+    x = torch.ones(n, device="cuda")
+    masks = []
+    for seed, stream in [(5, 0), (5, 1), (6, 0)]:
+        y, = launch(R.dropout("f32", n, p, stream_id=stream), [x, dev(np.array([seed, 0]), "i64")])
+        masks.append(y != 0)
+        assert abs(float(masks[-1].double().mean()) - (1 - p)) <= 6 * math.sqrt(p * (1 - p) / n)
+    for a, b in itertools.combinations(masks, 2):
+        both = float((a & b).double().mean())
+        assert abs(both - (1 - p) ** 2) <= 6 * math.sqrt((1 - p) ** 2 / n)
+
+
+# ---- block norms ----------------------------------------------------------------------------
+def norm_case(rng, dtype, rows, cols, params, layer, branch, post, pre, bias, groups):
+    v = {"x": rounded(rng, (rows, cols), dtype, 0.3, 2.0)}
+    if branch:
+        v["y"] = rounded(rng, (rows, cols), dtype, -0.4, 0.7)
+    if post:
+        v["w_post"] = rounded(rng, cols, params, 1.0, 0.3)
+        if bias:
+            v["b_post"] = rounded(rng, cols, params)
+    if groups:
+        v["gate"] = rounded(rng, (groups, cols), params, 0.5, 0.5)
+    if pre:
+        v["w_pre"] = rounded(rng, cols, params, 1.0, 0.3)
+        if bias:
+            v["b_pre"] = rounded(rng, cols, params)
+    return v
+
+
+SWITCHES = [  # layer, branch, post, pre, bias, groups, p, alpha
+    (False, True, True, True, False, 1, 0.0, 1.0),
+    (False, True, True, True, False, 3, 0.4, 0.5),
+    (True, True, True, True, True, 3, 0.2, 2.0),
+    (True, True, False, True, False, 0, 0.0, 1.0),
+    (False, True, True, False, True, 6, 0.3, 1.0),
+    (True, True, True, True, False, 0, 0.5, -1.5),
+    (False, True, False, False, False, 1, 0.1, 1.0),
+    (True, False, False, True, True, 0, 0.0, 1.0),
+]
+
+
+def run_norm(dtype, params, rows, cols, switch, skew=0, grad=True):
+    layer, branch, post, pre, bias, groups, p, alpha = switch
+    rng = np.random.default_rng(rows * 7919 + cols)
+    v = norm_case(rng, dtype, rows, cols, params, layer, branch, post, pre, bias, groups)
+    drop = (p, 77, 5, 3) if p else None
+    args = dict(norm="layer" if layer else "rms", eps=1e-5, branch=branch, post=post, pre=pre, bias=bias,
+                gate_groups=groups, residual_scale=alpha, dropout=p, stream_id=3, param_dtype=params)
+    seed = [dev(np.array([77, 5]), "i64")] if p else []
+    kinds = {"x": dtype, "y": dtype, "h": dtype, "dh": dtype, "du": dtype}
+    put = lambda d, names: [dev(d[n], kinds.get(n, params), skew if n in kinds else 0) for n in names if n in d]  # noqa: E731
+    out = launch(R.block_norm(dtype, rows, cols, **args),
+                 put(v, ["x", "y", "w_post", "b_post", "gate", "w_pre", "b_pre"]) + seed, skew)
+    want = ref.block_norm(v["x"], v.get("y"), v.get("w_post"), v.get("b_post"), v.get("gate"), v.get("w_pre"),
+                          v.get("b_pre"), layer, 1e-5, alpha, drop, post, pre)
+    names = (["h"] if branch else []) + (["u"] if pre else []) + (["stats_post"] if post else []) + (
+        ["stats_pre"] if pre else [])
+    for n, t in zip(names, out):
+        value, mag = want[n]
+        close(host(t, value.shape), value, ref.stored(value, mag, "f32" if n.startswith("stats") else dtype), n)
+    if not grad:
+        return
+    g = {n: rounded(rng, (rows, cols), dtype, 0.1, 0.5) for n in (["dh"] if branch else []) + (["du"] if pre else [])}
+    h = rounded(rng, (rows, cols), dtype, 0.3, 2.0)
+
+    def saved(x):
+        mean, rstd = ref.stats(x, layer, 1e-5)
+        s = np.stack([mean, rstd], 1) if layer else rstd[:, None]
+        return s.astype(np.float32).astype(np.float64)
+
+    sp, sr = saved(v["y"]) if post else None, saved(h) if pre else None
+    need_y = post or groups
+    ins = put(g, ["dh", "du"]) + (put({"h": h}, ["h"]) if pre else []) + (put(v, ["y"]) if need_y else [])
+    ins += put(v, ["w_post"] + (["b_post"] if groups else []) + ["gate", "w_pre"])
+    ins += [dev(s, "f32") for s in (sp, sr) if s is not None] + seed
+    out = launch(R.block_norm_grad(dtype, rows, cols, **args), ins, skew)
+    want = ref.block_norm_grad(g.get("dh"), g.get("du"), h, v.get("y"), v.get("w_post"), v.get("b_post"), v.get("gate"),
+                               v.get("w_pre"), sp, sr, layer, alpha, drop, bias)
+    names = ["dx"] + (["dy"] if branch else []) + (["dw_post"] if post else []) + (["db_post"] if post and bias else [])
+    names += (["dgate"] if groups else []) + (["dw_pre"] if pre else []) + (["db_pre"] if pre and bias else [])
+    assert len(names) == len(out)
+    for n, t in zip(names, out):
+        value, mag = want[n]
+        close(host(t, value.shape), value, ref.stored(value, mag, dtype if n in ("dx", "dy") else "f32"), n)
+
+
+@pytest.mark.parametrize("switch", SWITCHES)
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("rows,cols", [(6, 64), (36, 1000), (12, 257)])
+def test_block_norm_switches(device, switch, dtype, params, rows, cols):
+    run_norm(dtype, params, rows, cols, switch)
+
+
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 31, 255, 256, 264, 511, 512, 513, 1024, 2047, 4096, 4104, 8192, 8193,
+                                  20000, 32768, 32765])
+def test_block_norm_widths(device, dtype, params, cols):
+    run_norm(dtype, params, 6, cols, SWITCHES[2])
+
+
+@pytest.mark.parametrize("rows", [1, 2, 601, 5000])
+@pytest.mark.parametrize("cols", [96, 1000])
+def test_block_norm_row_counts(device, rows, cols):
+    run_norm("bf16", "f32", rows, cols, (False, True, True, True, False, 1, 0.2, 1.0))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [64, 520])
+def test_block_norm_unaligned_ports(device, dtype, cols):
+    run_norm(dtype, dtype, 6, cols, SWITCHES[2], skew=1)
+
+
+@pytest.mark.parametrize("rows,groups", [(40, 40), (200, 100), (64, 32), (66, 33)])
+def test_block_norm_many_groups(device, rows, groups):
+    run_norm("f32", "f32", rows, 130, (False, True, True, True, True, groups, 0.0, 1.0))
+
+
+def test_block_norm_no_rows(device):
+    out = launch(R.block_norm_grad("f32", 0, 40, gate_groups=0), [dev(np.zeros(0), "f32")] * 4 + [dev(np.ones(40), "f32")] * 2 +
+                 [dev(np.zeros(0), "f32")] * 2)
+    assert [t.numel() for t in out] == [0, 0, 40, 40] and all(bool((t == 0).all()) for t in out)
+    assert [t.numel() for t in launch(R.block_norm("f32", 0, 40), [dev(np.zeros(0), "f32")] * 2 + [dev(np.ones(40), "f32")] * 2)] == [0] * 4
+
+
+def test_block_norm_constant_rows(device):
+    """A layer norm of a constant row: variance 0, so the row is its bias; large means cost no precision."""
+    rows, cols = 4, 512
+    x = np.repeat(np.array([[0.0], [1.0], [4096.0], [-3.0e4]]), cols, 1)
+    u, s = launch(R.block_norm("f32", rows, cols, norm="layer", branch=False, bias=True),
+                  [dev(x, "f32"), dev(np.ones(cols), "f32"), dev(np.full(cols, 0.25), "f32")])
+    assert np.array_equal(host(u, (rows, cols)), np.full((rows, cols), 0.25))
+    assert np.array_equal(host(s, (rows, 2))[:, 0], x[:, 0])
+    rng = np.random.default_rng(0)
+    y = 1.0e4 + rng.standard_normal((rows, cols)).astype(np.float32)  # E[y^2] - mean^2 would lose all of this
+    y = y.astype(np.float32).astype(np.float64)
+    u, s = launch(R.block_norm("f32", rows, cols, norm="layer", branch=False),
+                  [dev(y, "f32"), dev(np.ones(cols), "f32")])
+    mean, rstd = ref.stats(y, True, 1e-6)
+    # y - mean is off by the mean's rounding, C u 1e4
+    assert np.abs(host(u, (rows, cols)) - (y - mean[:, None]) * rstd[:, None]).max() <= 2 * ref.C * ref.U * 1e4
+
+
+def test_block_norm_nan_and_inf_stay_in_their_row(device):
+    rng = np.random.default_rng(1)
+    rows, cols = 8, 300
+    x, y = rng.standard_normal((rows, cols)), rng.standard_normal((rows, cols))
+    x[2, 5], y[5, 7], y[6, 9] = np.nan, np.inf, np.nan
+    w = np.ones(cols)
+    h, u, _, _ = launch(R.block_norm("f32", rows, cols), [dev(a, "f32") for a in (x, y, w, w)])
+    bad = np.isnan(host(u, (rows, cols))).any(1)
+    assert bad.tolist() == [r in (2, 5, 6) for r in range(rows)]
+    assert np.isnan(host(h, (rows, cols))).any(1).tolist() == bad.tolist()
+
+
+# ---- bucketed-bias softmax -----------------------------------------------------------------------
+def run_softmax(dtype, shape, thresholds, both=True, scale=1.0, causal=False, lengths=None, offsets=None, p=0.0,
+                table_dtype="f32", skew=0, grad=True, s=None, seed=0):
+    rng = np.random.default_rng(seed + int(np.prod(shape)) + 13 * sum(shape))
+    nb, nh, nq, nk = shape
+    s = rounded(rng, shape, dtype, std=2.0 / scale) if s is None else s
+    buckets = (len(thresholds) + 1) * (2 if both else 1)
+    table = rounded(rng, (buckets, nh), table_dtype)
+    drop = (p, 99, 1234567890123, 4) if p else None
+    args = dict(bidirectional=both, scale=scale, causal=causal, lengths=lengths is not None,
+                offsets=offsets is not None, dropout=p, stream_id=4, table_dtype=table_dtype)
+    tail = [dev(np.array(v), "i32") for v in (lengths, offsets) if v is not None]
+    tail += [dev(np.array([99, 1234567890123]), "i64")] if p else []
+    ds, dt = dev(s, dtype, skew), dev(table, table_dtype)
+    f32scale = float(np.float32(scale))
+    out = launch(R.bias_softmax(dtype, *shape, thresholds, **args), [ds, dt] + tail, skew)
+    prob, ptol, lse, ltol = ref.bias_softmax(s, table, thresholds, both, f32scale, causal, lengths, offsets, drop)
+    tol = ptol + ref.HALF_ULP[dtype] * (prob + ptol) + ref.TINY[dtype]
+    close(host(out[0], shape), prob, tol, "p")
+    close(host(out[1], lse.shape), lse, ltol + ref.U * np.abs(np.where(np.isfinite(lse), lse, 0)), "lse")
+    if not grad:
+        return out
+    dp = rounded(rng, shape, dtype, std=0.5)
+    lse32 = lse.astype(np.float32)
+    out = launch(R.bias_softmax_grad(dtype, *shape, thresholds, **args),
+                 [ds, dev(dp, dtype, skew), dev(lse32, "f32"), dt] + tail, skew)
+    gs, gtol, gt, ttol = ref.bias_softmax_grad(s, dp, lse32.astype(np.float64), table, thresholds, both, f32scale,
+                                               causal, lengths, offsets, drop)
+    close(host(out[0], shape), gs, gtol + ref.HALF_ULP[dtype] * (np.abs(gs) + gtol) + ref.TINY[dtype], "ds")
+    close(host(out[1], gt.shape), gt, ttol + ref.U * np.abs(gt), "dtable")
+    return out
+
+
+TH = R.bucket_thresholds(32, 128, True)
+TH1 = R.bucket_thresholds(32, 128, False)
+
+
+@pytest.mark.parametrize("dtype,table", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("keys", [1, 2, 7, 8, 9, 63, 64, 129, 255, 256, 257, 500, 512, 1023, 1024, 1025, 2050, 4096])
+def test_bias_softmax_row_lengths(device, dtype, table, keys):
+    run_softmax(dtype, (2, 3, 5, keys), TH, table_dtype=table)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 2, 65, 65), (2, 4, 130, 130), (5, 3, 200, 37), (4, 4, 100, 301)])
+@pytest.mark.parametrize("both,causal,lens,p", [(True, False, True, 0.0), (False, True, False, 0.3), (True, False, False, 0.2),
+                                                (False, True, True, 0.0), (True, True, True, 0.1)])
+def test_bias_softmax_many_rows(device, dtype, shape, both, causal, lens, p):
+    """Enough rows for a warp each; lengths of zero and one among them."""
+    lengths = [[0, 1, shape[3], shape[3] // 2, 3][b % 5] for b in range(shape[0])] if lens else None
+    run_softmax(dtype, shape, TH if both else TH1, both, 0.25, causal, lengths, None, p)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("keys", [40, 777, 4096, 5001, 20000, 65536, 131065])
+def test_bias_softmax_single_tokens(device, dtype, keys):
+    batch, heads = (4, 3) if keys < 60000 else (1, 2)
+    lengths = [keys, 1, keys // 2 + 1, 0][:batch]
+    run_softmax(dtype, (batch, heads, 1, keys), TH1, False, 0.125, False, lengths, [n - 1 for n in lengths])
+
+
+def test_bias_softmax_longest_rows(device):
+    run_softmax("bf16", (1, 2, 1, 131072), TH, offsets=[131071])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("keys", [48, 515])
+def test_bias_softmax_unaligned_ports(device, dtype, keys):
+    run_softmax(dtype, (3, 2, 40, keys), TH, lengths=[keys, 5, 0], p=0.2, skew=1)
+
+
+@pytest.mark.parametrize("offsets", [[0, 100, -5], [-200, 7, 2 ** 31 - 1], [-2 ** 31, 40, 3]])
+@pytest.mark.parametrize("causal", [False, True])
+def test_bias_softmax_offsets(device, offsets, causal):
+    """Queries far before, within and far after the keys; causal rows without any key."""
+    run_softmax("f32", (3, 2, 9, 50), TH, True, 1.0, causal, None, offsets)
+
+
+@pytest.mark.parametrize("thresholds,both", [([1], True), ([1], False), ([5, 5, 9], True), ([4096], False), ([4096], True),
+                                             (list(range(1, 256)), True), (R.bucket_thresholds(320, 800, True), True)])
+def test_bias_softmax_bucket_shapes(device, thresholds, both):
+    run_softmax("f32", (2, 2, 33, 300), thresholds, both)
+    run_softmax("bf16", (8, 4, 60, 200), thresholds, both, p=0.1)
+
+
+def test_bias_softmax_extreme_scores(device):
+    """Rows of -inf, of the type's lowest value, one +inf, NaN in masked and in visible places."""
+    shape = (1, 1, 6, 40)
+    for dtype, low in [("f16", -65504.0), ("f32", float(np.finfo(np.float32).min)), ("bf16", -3.3895e38)]:
+        s = np.zeros(shape)
+        s[0, 0, 0] = -np.inf
+        s[0, 0, 1] = low
+        s[0, 0, 2, 3] = -np.inf
+        s[0, 0, 3, 30:] = np.nan      # behind the length
+        s[0, 0, 4, 2] = np.nan        # seen
+        s[0, 0, 5, 35] = np.inf       # behind the length
+        lengths = dev(np.array([30]), "i32")
+        table = np.zeros((32, 1))
+        p, lse = launch(R.bias_softmax(dtype, *shape, TH, lengths=True), [dev(s, dtype), dev(table, "f32"), lengths])
+        p, lse = host(p, shape)[0, 0], host(lse, 6)
+        u = ref.HALF_ULP[dtype] + ref.C * ref.U
+        assert (p[0] == 0).all() and lse[0] == -np.inf
+        for r, n in ((1, 30), (2, 29), (3, 30), (5, 30)):
+            nz = p[r, :30][np.arange(30) != 3] if r == 2 else p[r, :30]
+            assert np.abs(nz * n - 1).max() <= 2 * u
+            assert (p[r, 30:] == 0).all()
+        assert p[2, 3] == 0 and np.isnan(p[4, :30]).all() and (p[4, 30:] == 0).all()
+        dp = np.ones(shape)
+        dp[0, 0, 3, 30:] = np.nan
+        ds, dt = launch(R.bias_softmax_grad(dtype, *shape, TH, lengths=True),
+                        [dev(s[:, :, [0, 1, 2, 3, 3, 5]], dtype), dev(dp[:, :, [0, 1, 2, 3, 3, 5]], dtype),
+                         dev(np.where(np.isnan(lse), lse[3], lse)[[0, 1, 2, 3, 3, 5]], "f32"), dev(table, "f32"), lengths])
+        ds = host(ds, shape)[0, 0]
+        assert (ds[0] == 0).all() and np.isfinite(ds).all() and (ds[:, 30:] == 0).all() and bool(torch.isfinite(dt).all())
+
+
+def test_bias_softmax_no_keys_and_no_rows(device):
+    p, lse = launch(R.bias_softmax("f32", 2, 3, 4, 0, TH), [dev(np.zeros(0), "f32"), dev(np.zeros((32, 3)), "f32")])
+    assert p.numel() == 0 and bool((lse == -math.inf).all())
+    for shape in [(0, 3, 4, 5), (2, 3, 0, 5), (2, 3, 4, 0)]:
+        rows = shape[0] * shape[1] * shape[2]
+        n = rows * shape[3]
+        ds, dt = launch(R.bias_softmax_grad("f32", *shape, TH),
+                        [dev(np.zeros(n), "f32"), dev(np.zeros(n), "f32"), dev(np.full(rows, -math.inf), "f32"), dev(np.zeros((32, 3)), "f32")])
+        assert dt.numel() == 96 and bool((dt == 0).all())
+
+
+# ---- gradients against differences of the kernels' own formulas --------------------------------------
+def test_gradients_against_differences(device):
+    """The kernels' f32 gradients along random directions against central differences of the 64-bit forms."""
+    rng = np.random.default_rng(11)
+    rows, cols = 12, 70
+    for layer in (False, True):
+        v = norm_case(rng, "f32", rows, cols, "f32", layer, True, True, True, True, 3)
+        dh, du = rounded(rng, (rows, cols), "f32"), rounded(rng, (rows, cols), "f32")
+        drop = (0.25, 8, 9, 0)
+        names = ["x", "y", "w_post", "b_post", "gate", "w_pre", "b_pre"]
+        f = lambda a: ref.block_norm(*a, layer, 1e-5, 0.7, drop, True, True)  # noqa: E731
+        base = [v[n] for n in names]
+        o = f(base)
+        stats = [o["stats_post"][0], o["stats_pre"][0]]
+        ins = [dev(a, "f32") for a in (dh, du, o["h"][0], v["y"], v["w_post"], v["b_post"], v["gate"], v["w_pre"], *stats)]
+        g = launch(R.block_norm_grad("f32", rows, cols, norm="layer" if layer else "rms", eps=1e-5, bias=True,
+                                     gate_groups=3, residual_scale=0.7, dropout=0.25), ins + [dev(np.array([8, 9]), "i64")])
+        for k, (a, t) in enumerate(zip(base, g)):
+            d = rng.standard_normal(a.shape)
+            loss = lambda e: sum((f([b + e * d if j == k else b for j, b in enumerate(base)])[n][0] * w).sum()  # noqa: E731
+                                 for n, w in (("h", dh), ("u", du)))
+            num = (loss(1e-4) - loss(-1e-4)) / 2e-4
+            terms = host(t, a.shape) * d
+            # third-order differences ~1e-7; the kernel's 32-bit sums
+            assert abs(num - terms.sum()) <= 1e-5 * np.abs(terms).sum() + 1e-5, names[k]
+    shape = (2, 2, 6, 20)
+    th = [1, 2, 4, 8]
+    s, dp = rounded(rng, shape, "f32"), rounded(rng, shape, "f32")
+    table = rounded(rng, (10, 2), "f32")
+    call = dict(both=True, scale=0.5, causal=False, lengths=[20, 9], offsets=None)
+    drop = (0.2, 8, 9, 0)
+    lse = ref.bias_softmax(s, table, th, drop=drop, **call)[2]
+    ds, dt = launch(R.bias_softmax_grad("f32", *shape, th, scale=0.5, lengths=True, dropout=0.2),
+                    [dev(a, "f32") for a in (s, dp, lse, table)] + [dev(np.array([20, 9]), "i32"), dev(np.array([8, 9]), "i64")])
+    for a, t, at in ((s, ds, 0), (table, dt, 1)):
+        d = rng.standard_normal(a.shape)
+        loss = lambda e: (ref.bias_softmax(s + e * d if at == 0 else s, table + e * d if at == 1 else table, th,  # noqa: E731
+                                           drop=drop, **call)[0] * dp).sum()
+        num = (loss(1e-4) - loss(-1e-4)) / 2e-4
+        terms = host(t, a.shape) * d
+        assert abs(num - terms.sum()) <= 1e-5 * np.abs(terms).sum() + 1e-5
+
+
+# ---- determinism, streams, graphs, programs, large offsets ---------------------------------------------
+def grad_calls():
+    rng = np.random.default_rng(2)
+    rows, cols = 3000, 264
+    a = lambda *s: dev(rng.standard_normal(s), "bf16")  # noqa: E731
+    f = lambda *s: dev(rng.standard_normal(s), "f32")  # noqa: E731
+    seed = dev(np.array([4, 4]), "i64")
+    yield (R.block_norm_grad("bf16", rows, cols, gate_groups=2, dropout=0.1),
+           [a(rows, cols) for _ in range(4)] + [f(cols), f(2, cols), f(cols), f(rows).abs(), f(rows).abs(), seed])
+    yield (R.bias_softmax_grad("bf16", 6, 5, 90, 90, TH, dropout=0.1),
+           [a(6, 5, 90, 90), a(6, 5, 90, 90), f(6, 5, 90).abs() + 5, f(32, 5), seed])
+
+
+def test_gradients_are_deterministic_on_any_stream(device):
+    for recipe, ins in grad_calls():
+        first = launch(recipe, ins)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            again = launch(recipe, ins, stream=side)
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(first, again))
+
+
+def test_graph_replay_draws_new_masks(device):
+    n = 10_000
+    x, seed = torch.ones(n, device="cuda"), dev(np.array([1, 0]), "i64")
+    y = torch.empty_like(x)
+    plan = ask_b200.Plan(R.dropout("f32", n, 0.5), device=0)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        plan.launch([x, seed], [y], None, stream)
+        seed[1] += (n + 3) // 4
+    for step in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.cpu(), dropout_exact(np.ones(n), None, 0.5, 1, step * 2500, 0, "f32"))
+
+
+def test_missing_scratch_and_ports_are_errors(device):
+    for recipe, ins in grad_calls():
+        plan = ask_b200.Plan(recipe, device=0)
+        outs = [torch.empty(p["elements"], dtype=TORCH[p["element_type"]], device="cuda")
+                for p in plan.describe()["port_map"][plan.n_inputs:]]
+        with pytest.raises(ask_b200.AskB200Error, match="scratch"):
+            plan.launch(ins, outs, None)
+        with pytest.raises(ask_b200.AskB200Error, match="ports"):
+            plan.launch(ins[:-1], outs, None)
+        with pytest.raises(ask_b200.AskB200Error, match="NULL"):
+            plan.launch([None] + ins[1:], outs, None)
+    with pytest.raises(ask_b200.AskB200Error, match="reduce"):
+        plan.launch_noalloc(ins, outs)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_runtime_program_of_block_operators(device, graph):
+    """scores -> bias_softmax, and its gradient, as steps of one program with internal buffers and scratch."""
+    from ask_b200 import runtime as rt
+    shape, n, rows = (2, 3, 40, 40), 9600, 240
+    rng = np.random.default_rng(3)
+    s, dp, table = rounded(rng, shape, "f32"), rounded(rng, shape, "f32"), rounded(rng, (32, 3), "f32")
+    sess = rt.Session.create(0)
+    # buffers: 0 s, 1 table, 2 dp, 3 p, 4 lse (internal), 5 ds, 6 dtable
+    prog = sess.prepareProgram([4 * n, 4 * 96, 4 * n, 4 * n, 4 * rows, 4 * n, 4 * 96], [0, 1, 2], [3, 5, 6],
+                               [rt.PlanStep(R.bias_softmax("f32", *shape, TH), [0, 1], [3, 4]),
+                                rt.PlanStep(R.bias_softmax_grad("f32", *shape, TH), [0, 2, 4, 1], [5, 6])], graph=graph)
+    ts = [dev(a, "f32") for a in (s, table, dp)]
+    torch.cuda.synchronize()
+    for _ in range(2):
+        outs, event = prog.run([sess.importTensor(t, readonly=True) for t in ts])
+        event.wait()
+        p, ptol, lse, _ = ref.bias_softmax(s, table, TH, True, 1.0, False, None, None, None)
+        close(np.frombuffer(outs[0].copyToHost(), np.float32).reshape(shape).astype(float), p, ptol + ref.U * p, "p")
+        ds, gtol, dt, ttol = ref.bias_softmax_grad(s, dp, lse, table, TH, True, 1.0, False, None, None, None)
+        # lse comes from the step before: its error scales P
+        close(np.frombuffer(outs[1].copyToHost(), np.float32).reshape(shape).astype(float), ds, 2 * gtol, "ds")
+        close(np.frombuffer(outs[2].copyToHost(), np.float32).reshape(32, 3).astype(float), dt, 2 * ttol, "dtable")
+
+
+def test_offsets_past_32_bits(device):
+    """Tensors of more than 2^31 elements: the last elements, and the bytes behind them, are right."""
+    n = 2 ** 31 + 4099
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = torch.empty_like(x)
+    seed = dev(np.array([1, 2 ** 40]), "i64")
+    ask_b200.Plan(R.dropout("bf16", n, 0.5), 0).launch([x, seed], [y], None, torch.cuda.current_stream())
+    first = (n - 5000) // 4 * 4
+    keep = ref.keep_mask(0.5, 1, 2 ** 40 + first // 4, 0, (n - first,))
+    assert np.array_equal(y[first:].float().cpu().numpy(), 2.0 * keep)
+    # norm of rows whose last starts beyond 2^31 elements; only that row holds other values
+    rows, cols = 65538, 32768
+    x = torch.ones(rows * cols, dtype=torch.bfloat16, device="cuda")
+    x[-cols:] = torch.arange(cols, device="cuda").to(torch.bfloat16)
+    u, s = torch.empty_like(x), torch.empty(rows, device="cuda")
+    w = torch.ones(cols, device="cuda")
+    ask_b200.Plan(R.block_norm("bf16", rows, cols, branch=False, eps=0.0), 0).launch([x, w], [u, s], None, torch.cuda.current_stream())
+    v = x[-cols:].double().cpu().numpy()
+    r = 1 / math.sqrt((v * v).mean())
+    got = u[-cols:].double().cpu().numpy()
+    assert np.abs(got - v * r).max() <= (2.0 ** -8 + 1e-5) * np.abs(v * r).max()
+    assert abs(float(s[-1]) - r) <= 64 * ref.U * r and float(s[0]) == 1.0 and bool((u[:cols] == 1).all())
+    del x, u, y
+    # scores of a long cache: rows up to element 2^31 + ...
+    shape = (2, 131, 64, 131072 - 128)
+    total = int(np.prod(shape))
+    assert total > 2 ** 31
+    sc = torch.zeros(total, dtype=torch.float16, device="cuda")
+    p, lse = torch.full_like(sc, 3.0), torch.empty(total // shape[3], device="cuda")
+    table = torch.zeros(32 * shape[1], device="cuda")
+    ask_b200.Plan(R.bias_softmax("f16", *shape, TH, lengths=True), 0).launch(
+        [sc, table, dev(np.array([0, 1000]), "i32")], [p, lse], None, torch.cuda.current_stream())
+    last = p[-shape[3]:]
+    assert bool((last[1000:] == 0).all()) and abs(float(last[999]) * 1000 - 1) <= 2.0 ** -10
+    assert abs(float(lse[-1]) - math.log(1000)) <= 1e-5 and float(lse[0]) == -math.inf
+    assert bool((p[:shape[3]] == 0).all())
