@@ -4,6 +4,7 @@
 #pragma once
 
 #include "ask_numerics.cuh"
+#include "kernels.h"
 #include "pair_f32.cuh"
 #include "vec_io.cuh"
 
@@ -50,27 +51,82 @@ __device__ __forceinline__ uint4 act_narrow(const float* v) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What a thread holds of a row before it is widened: V elements, 16 bytes or one.
+// The 16 bytes at byte `shift` (0 to 15, a multiple of the element size) of
+// two neighbouring 16-byte words.
+template <int T>
+__device__ __forceinline__ uint4 unit_at(const uint4& a, const uint4& b, uint32_t shift) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int k = 0; k < 6; ++k) w[k] = (shift & 8u) ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) w[k] = (shift & 4u) ? w[k + 1] : w[k];
+  if constexpr (T != kF32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2u) * 8u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The aligned 16 bytes at `at`, of which only those in [begin, end) may be read;
+// the others are 0.
+template <int T>
+__device__ __forceinline__ uint4 load_part(const char* at, const char* begin, const char* end) {
+  constexpr int kBytes = dtype_bytes(T), kPerWord = 4 / kBytes;
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int k = 0; k < 16 / kBytes; ++k) {
+    const char* e = at + k * kBytes;
+    if (e < begin || e >= end) continue;
+    const uint32_t bits = kBytes == 4 ? __ldg(reinterpret_cast<const uint32_t*>(e))
+                                      : uint32_t(__ldg(reinterpret_cast<const unsigned short*>(e)));
+    w[k / kPerWord] |= bits << (8 * kBytes * (k % kPerWord));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Stores a warp's units (16 bytes a lane, lane after lane) to rows that start
+// anywhere: lane k puts together the aligned word that its unit begins in from
+// lane k - 1's unit and its own, so only the ends of a run of lanes are stored
+// element by element.  `p`: where this lane's unit belongs; `n` of its elements
+// exist (0: none); `first`, `last`: the run begins or ends with this lane.  All
+// lanes of the warp call it.
+template <int T>
+__device__ __forceinline__ void store_anywhere(char* p, const uint4& own, int n, bool first, bool last) {
+  constexpr int kBytes = dtype_bytes(T);
+  const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+  uint4 prev;
+  prev.x = __shfl_up_sync(0xffffffffu, own.x, 1);
+  prev.y = __shfl_up_sync(0xffffffffu, own.y, 1);
+  prev.z = __shfl_up_sync(0xffffffffu, own.z, 1);
+  prev.w = __shfl_up_sync(0xffffffffu, own.w, 1);
+  const int head = int(16u - shift) / kBytes;  // own elements in the word that the unit begins in
+  // a unit with elements follows whole units of its run
+  const bool whole = shift == 0 ? n == 16 / kBytes : !first && n >= head;
+  const bool next_whole = __shfl_down_sync(0xffffffffu, int(whole), 1) && !last;
+  if (whole) st_stream_v4(p - shift, shift == 0 ? own : unit_at<T>(prev, own, 16u - shift));
+  if (n > 0 && (!whole || (shift != 0 && !next_whole))) {
+    const uint32_t w[4] = {own.x, own.y, own.z, own.w};
+#pragma unroll
+    for (int k = 0; k < 16 / kBytes; ++k) {
+      if (k >= n || (k < head ? whole : next_whole)) continue;
+      if constexpr (kBytes == 4) reinterpret_cast<uint32_t*>(p)[k] = w[k];
+      else reinterpret_cast<uint16_t*>(p)[k] = uint16_t(w[k / 2] >> (16 * (k % 2)));
+    }
+  }
+}
+
+// What a thread holds of a row before it is widened: 16 bytes.
 template <int T, int V>
 struct ActRaw {
+  static_assert(V == act_vec<T>(), "16 bytes");
   uint4 r;
   __device__ __forceinline__ void load(const void* p, uint64_t i) {
     r = ld_stream_v4(static_cast<const char*>(p) + i * dtype_bytes(T));
   }
-  __device__ __forceinline__ void zero() { r = make_uint4(0u, 0u, 0u, 0u); }
   __device__ __forceinline__ void widen(float* v) const { act_widen<T>(r, v); }
-};
-template <int T>
-struct ActRaw<T, 1> {
-  float f;
-  __device__ __forceinline__ void load(const void* p, uint64_t i) { f = act_load<T>(p, i); }
-  __device__ __forceinline__ void zero() { f = 0.0f; }
-  __device__ __forceinline__ void widen(float* v) const { v[0] = f; }
 };
 template <int T, int V>
 __device__ __forceinline__ void act_put(void* p, uint64_t i, const float* v) {
-  if constexpr (V == 1) act_store<T>(p, i, v[0]);
-  else st_stream_v4(static_cast<char*>(p) + i * dtype_bytes(T), act_narrow<T>(v));
+  st_stream_v4(static_cast<char*>(p) + i * dtype_bytes(T), act_narrow<T>(v));
 }
 
 // V parameters (weights, gates) of run-time type starting at column c: read

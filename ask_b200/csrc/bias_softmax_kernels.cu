@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   __shared__ TeamRecords<1> sh;
   __shared__ float ends[2][kTeamThreads / 32];
   const bool warp_teams = a.shape.warp_teams;
-  const Team t = team_of(warp_teams);
+  const Team t = team_of(a.shape.warp_teams);
   const Window win = window_of(a);
   Task task = task_of(a, t);
   const int teams = warp_teams ? int(blockDim.x >> 5) : 1;
@@ -405,7 +405,7 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   const uint64_t span = keys % v ? keys + v - 1 : keys;
   TeamShape s{0, kWarpTeamThreads, 1, 32};
   if (rows >= uint64_t(sms) * 8 && span <= 32 * 32) {
-    s.warp_teams = 1;
+    s.warp_teams = 32;
     s.elems = span <= 32 * 8 ? 8 : span <= 32 * 16 ? 16 : 32;
     return s;
   }

@@ -2,9 +2,9 @@
 // stored; the backward pass is the same map of dy (philox.cuh has the rule).
 //
 // Bound: HBM, 2 (3 with a residual) elements moved for each one computed; the
-// generator costs 5 widening products an element (20 for four), which at two
-// bytes an element is close enough to the memory time that the integer work
-// has to overlap the loads: every thread keeps kUnits 16-byte units in flight.
+// generator's products (philox.cuh) take about as long as HBM needs for 2-byte
+// elements and half as long as for 4-byte ones, so the next units' loads are
+// issued before this one's integer work.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -18,7 +18,14 @@ namespace askb {
 
 namespace {
 
-constexpr int kUnits = 2;
+// 16-byte units a thread has in flight, and CTAs an SM the registers are held
+// to.  The generator's work is what 2-byte elements wait for, so they take
+// four units (eight blocks side by side) and all the registers that takes; the
+// others wait for memory.
+template <int T, bool kRes>
+constexpr int units_in_flight() { return act_vec<T>() == 8 && !kRes ? 4 : 2; }
+template <int T, bool kRes>
+constexpr int ctas_per_sm() { return act_vec<T>() == 8 ? (kRes ? 3 : 1) : 4; }
 
 template <int T>
 __device__ __forceinline__ void load_elems(const void* p, uint64_t i, int n, float* v) {
@@ -27,14 +34,14 @@ __device__ __forceinline__ void load_elems(const void* p, uint64_t i, int n, flo
 }
 
 template <int T, bool kRes, bool kAligned>
-__global__ void __launch_bounds__(kDropThreads) dropout_kernel(const DropoutArgs a) {
+__global__ void __launch_bounds__(kDropThreads, ctas_per_sm<T, kRes>()) dropout_kernel(const DropoutArgs a) {
   constexpr int V = act_vec<T>();
   pdl_enter();
   const DropRun run = drop_run(a.drop, a.seed);
   const uint64_t units = a.count / V, stride = uint64_t(gridDim.x) * kDropThreads;
   uint64_t u = uint64_t(blockIdx.x) * kDropThreads + threadIdx.x;
   auto finish = [&](uint64_t at, int n, float* v, const float* r) {
-    if (run.scale != 0.0f) drop_unit<V>(run, at, v);
+    if (a.drop.on) drop_unit<V>(run, at, v);
     if constexpr (kRes) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = __fadd_rn(v[j], r[j]);
@@ -48,20 +55,31 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const DropoutArgs
     }
   };
   if constexpr (kAligned) {
-    for (; u + (kUnits - 1) * stride < units; u += kUnits * stride) {
-      ActRaw<T, V> x[kUnits], r[kUnits];
+    // U units a step, the next step's loads issued before this one's math
+    constexpr int U = units_in_flight<T, kRes>();
+    ActRaw<T, V> x[U], r[U];
+    auto fetch = [&](uint64_t from) {
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        x[k].load(a.x, (u + k * stride) * V);
-        if constexpr (kRes) r[k].load(a.residual, (u + k * stride) * V);
+      for (int k = 0; k < U; ++k) {
+        x[k].load(a.x, (from + k * stride) * V);
+        if constexpr (kRes) r[k].load(a.residual, (from + k * stride) * V);
       }
+    };
+    bool more = u + (U - 1) * stride < units;
+    if (more) fetch(u);
+    while (more) {
+      float v[U][V], w[U][V];
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        float v[V], w[V];
-        x[k].widen(v);
-        if constexpr (kRes) r[k].widen(w);
-        finish((u + k * stride) * V, V, v, w);
+      for (int k = 0; k < U; ++k) {
+        x[k].widen(v[k]);
+        if constexpr (kRes) r[k].widen(w[k]);
       }
+      const uint64_t now = u;
+      u += U * stride;
+      more = u + (U - 1) * stride < units;
+      if (more) fetch(u);
+#pragma unroll
+      for (int k = 0; k < U; ++k) finish((now + k * stride) * V, V, v[k], w[k]);
     }
   }
   // the rest, the last unit possibly cut short

@@ -212,7 +212,7 @@ constexpr int kDropThreads = 256;
 
 // How a row's threads are laid out: see row_team.cuh.
 struct TeamShape {
-  int warp_teams;  // every warp takes a row of its own
+  int warp_teams;  // lanes of a warp that take a row (4 to 32), 0: the whole CTA or cluster
   int threads;     // of a CTA
   int ctas;        // of a row's cluster (1: no cluster)
   int elems;       // row elements a thread holds
@@ -243,7 +243,7 @@ struct NormArgs {
   TeamShape shape;
 };
 constexpr int kNormMaxCols = 32768;
-TeamShape norm_shape(uint64_t cols, bool grad);
+TeamShape norm_shape(uint64_t cols, int type);
 // Row sums the gradient keeps for each column: of B*yhat, B, du*hhat, du.
 struct NormSums {
   bool t, s, p, q;
@@ -251,8 +251,11 @@ struct NormSums {
 };
 NormSums norm_sums(const NormArgs& a);
 cudaError_t norm_occupancy(const NormArgs& a, bool grad, int* blocks_per_sm);
-cudaError_t norm_launch(const NormArgs& a, bool vec, int grid, cudaStream_t stream);
-cudaError_t norm_grad_launch(const NormArgs& a, bool vec, cudaStream_t stream);
+// `aligned`: every row of every port starts on a 16-byte boundary.
+cudaError_t norm_launch(const NormArgs& a, bool aligned, int grid, cudaStream_t stream);
+cudaError_t norm_grad_launch(const NormArgs& a, bool aligned, cudaStream_t stream);
+// Rows a CTA works on at once.
+inline int team_count(const TeamShape& s) { return s.warp_teams ? s.threads / s.warp_teams : 1; }
 
 // Softmax over biased scores (bias_softmax_kernels.cu).  s, p, dp, ds are
 // [batch, heads, queries, keys] of `type`, table [buckets, heads] of

@@ -34,283 +34,577 @@ namespace askb {
 namespace {
 
 constexpr int kWarpTeamThreads = 256;
+constexpr int kElems = 16;  // row elements a thread holds
 
-// Mean and 1 / sqrt(variance + eps) of the team's row; v is zero past cols.
-template <int E, int V, class Valid>
-__device__ __forceinline__ void row_stats(const Team& t, TeamRecords<1>& sh_mean, TeamRecords<1>& sh_sq, int parity,
-                                          bool layer, float inv_cols, float eps, const float (&v)[E], Valid valid,
-                                          float& mean, float& rstd) {
-  mean = 0.0f;
-  if (layer) {
-    float s[1] = {0.0f};
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += v[e];
-    team_sum<1>(t, sh_mean, parity, s);
-    mean = s[0] * inv_cols;
-  }
-  float s[1] = {0.0f};
-#pragma unroll
-  for (int q = 0; q < E / V; ++q) {
-    const float m = valid(q) ? mean : 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = v[q * V + j] - m;
-      s[0] = __fmaf_rn(d, d, s[0]);
-    }
-  }
-  team_sum<1>(t, sh_sq, parity, s);
-  rstd = __frsqrt_rn(__fmaf_rn(s[0], inv_cols, eps));
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+__device__ __forceinline__ float sum2(uint64_t v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return lo + hi;
 }
 
-template <int T, int V, int E>
-__global__ void __launch_bounds__(kTeamThreads) norm_rows_kernel(const NormArgs a) {
-  constexpr int Q = E / V;
+// A row array in flight: every thread copies the 16-byte words of its own
+// units into its own places of a ring in shared memory (cp.async) and reads
+// them back, so no barrier is needed, rows are fetched kStages - 1 ahead, and no
+// register holds what is on its way.  Where rows start anywhere (kAnywhere) a
+// unit spans two words.
+template <int T, bool kAnywhere>
+struct Ring {
+  static constexpr int V = act_vec<T>(), Q = kElems / V, W = kAnywhere ? 2 : 1;
+  static constexpr int kWords = Q * W;  // 16-byte words of one thread, array and stage
+};
+
+// Shared memory by its 32-bit address.
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void copy_to_shared(uint32_t at, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+}
+
+// The team's columns of a row, as the thread holds them: units of 16 bytes, as
+// f32 pairs.  A row is named by the byte offset of this thread's first column.
+template <int T, bool kAnywhere>
+struct Columns {
+  static constexpr int E = kElems, V = act_vec<T>(), Q = E / V, P = E / 2, B = dtype_bytes(T);
+  uint32_t first, step;  // column of unit q: first + q * step
+  uint32_t cols, pitch;  // pitch: between a thread's words in shared memory
+  __device__ __forceinline__ Columns(const Team& t, const NormArgs& a)
+      : first((t.rank * uint32_t(Q) * t.threads + t.tid) * uint32_t(V)), step(t.threads * uint32_t(V)), cols(a.cols),
+        pitch(blockDim.x * 16) {}
+  __device__ __forceinline__ uint32_t at(int q) const { return first + uint32_t(q) * step; }
+  __device__ __forceinline__ bool in(int q) const { return at(q) < cols; }
+  __device__ __forceinline__ int count(int q) const { return in(q) ? int(min(cols - at(q), uint32_t(V))) : 0; }
+  __device__ __forceinline__ uint64_t offset(uint64_t row) const { return (row * cols + first) * uint64_t(B); }
+  __device__ __forceinline__ const char* unit(const void* p, uint64_t off, int q) const {
+    return static_cast<const char*>(p) + off + uint64_t(uint32_t(q) * step * uint32_t(B));
+  }
+
+  // `slot`: this thread's words of the array in a stage.  What no column fills
+  // is zeroed once, by clear().
+  __device__ __forceinline__ void fetch(const void* p, uint64_t off, uint64_t bytes, uint32_t slot) const {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (!in(q)) continue;
+      const char* from = unit(p, off, q);
+      if constexpr (!kAnywhere) {
+        copy_to_shared(slot + uint32_t(q) * pitch, from);
+      } else {
+        const char* word = from - (reinterpret_cast<uintptr_t>(from) & 15u);
+        const char* begin = static_cast<const char*>(p);
+        const char* last = from + count(q) * B;  // the unit's elements end here
+#pragma unroll
+        for (int k = 0; k < 2; ++k, word += 16) {
+          const uint32_t to = slot + uint32_t(q * 2 + k) * pitch;
+          if (word >= last) continue;  // nothing of the unit in it
+          if (word >= begin && word + 16 <= begin + bytes) copy_to_shared(to, word);
+          else st_shared(to, load_part<T>(word, begin, begin + bytes));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void clear(uint32_t slot) const {
+    if constexpr (!kAnywhere) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        if (!in(q)) st_shared(slot + uint32_t(q) * pitch, make_uint4(0u, 0u, 0u, 0u));
+    }
+  }
+  __device__ __forceinline__ void read(uint32_t slot, const void* p, uint64_t off, uint64_t (&v)[P]) const {
+    float f[E];
+    const uint32_t shift = (uint32_t(reinterpret_cast<uintptr_t>(p)) + uint32_t(off)) & 15u;  // of all units: they are words apart
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if constexpr (!kAnywhere) {
+        act_widen<T>(ld_shared(slot + uint32_t(q) * pitch), f + q * V);
+      } else {
+        act_widen<T>(unit_at<T>(ld_shared(slot + uint32_t(2 * q) * pitch), ld_shared(slot + uint32_t(2 * q + 1) * pitch), shift),
+                     f + q * V);
+        const int n = count(q);
+        if (n < V) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[q * V + j] = j < n ? f[q * V + j] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
+  }
+  __device__ __forceinline__ void put(const Team& t, void* p, uint64_t off, bool on, const uint64_t (&v)[P]) const {
+    float f[E];
+    unpack(v, f);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      char* to = const_cast<char*>(unit(p, off, q));
+      if constexpr (kAnywhere) {
+        const uint32_t place = t.lane & (t.lanes - 1);
+        store_anywhere<T>(to, act_narrow<T>(f + q * V), on ? count(q) : 0, place == 0, place == t.lanes - 1);
+      } else if (on && in(q)) {
+        st_stream_v4(to, act_narrow<T>(f + q * V));
+      }
+    }
+  }
+  __device__ __forceinline__ static void unpack(const uint64_t (&v)[P], float* f) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) unpack2(v[k], f[2 * k], f[2 * k + 1]);
+  }
+  // parameters of these columns, `fill` where the step has none; 0 past the row
+  __device__ __forceinline__ void params(const void* p, int type, uint64_t offset, float fill, float* f) const {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int n = count(q);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[q * V + j] = j < n ? fill : 0.0f;
+      if (!p) continue;
+      if (!kAnywhere && n) {
+        param_load<V>(p, type, offset + at(q), f + q * V);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < n) param_load<1>(p, type, offset + at(q) + j, f + q * V + j);
+      }
+    }
+  }
+  // v - mean where there is a column; the rest stays 0
+  __device__ __forceinline__ void center(float mean, uint64_t (&v)[P]) const {
+    float f[E];
+    unpack(v, f);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int n = count(q);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[q * V + j] -= (kAnywhere ? j < n : n != 0) ? mean : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
+  }
+  // zero where dropped; the scale is folded into what the values meet next.
+  // Units past the row hold zeros, whatever is drawn for them.
+  __device__ __forceinline__ void drop(const DropRun& run, uint64_t off, uint64_t (&v)[P]) const {
+    float f[E];
+    unpack(v, f);
+    uint64_t i[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) i[q] = off / B + uint32_t(q) * step;
+    bool keep[E];
+    drop_keep<Q, V, kAnywhere>(run, i, keep);
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = pack2(keep[2 * k] ? f[2 * k] : 0.0f, keep[2 * k + 1] ? f[2 * k + 1] : 0.0f);
+  }
+};
+
+// A thread's parameters, in its own words of shared memory.
+struct ParamSlot {
+  uint32_t at, pitch;
+  __device__ __forceinline__ void write(const float (&f)[kElems]) const {
+#pragma unroll
+    for (int k = 0; k < kElems / 4; ++k)
+      st_shared(at + uint32_t(k) * pitch, make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]),
+                                                     __float_as_uint(f[4 * k + 2]), __float_as_uint(f[4 * k + 3])));
+  }
+  __device__ __forceinline__ void pair(int k, uint64_t& lo, uint64_t& hi) const {  // elements 4k .. 4k + 3
+    asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(at + uint32_t(k) * pitch) : "memory");
+  }
+};
+
+template <int N>
+__device__ __forceinline__ float dot(const uint64_t (&a)[N], const uint64_t (&b)[N]) {
+  uint64_t s = mul2(a[0], b[0]), t = N > 1 ? mul2(a[1], b[1]) : 0;
+#pragma unroll
+  for (int k = 2; k < N; k += 2) {
+    s = fma2(a[k], b[k], s);
+    if (k + 1 < N) t = fma2(a[k + 1], b[k + 1], t);
+  }
+  return sum2(N > 1 ? add2(s, t) : s);
+}
+template <int N>
+__device__ __forceinline__ float total(const uint64_t (&a)[N]) {
+  uint64_t s = a[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) s = add2(s, a[k]);
+  return sum2(s);
+}
+
+// Centres the row (layer norm) and gives its mean and 1 / sqrt(variance + eps).
+template <int T, bool kAnywhere>
+__device__ __forceinline__ void row_stats(const Team& t, const Columns<T, kAnywhere>& c, TeamRecords<1>& sh_mean,
+                                          TeamRecords<1>& sh_sq, int parity, bool layer, float inv_cols, float eps,
+                                          uint64_t (&v)[kElems / 2], float& mean, float& rstd) {
+  mean = 0.0f;
+  if (layer) {
+    float s[1] = {total(v)};
+    team_sum<1>(t, sh_mean, parity, s);
+    mean = s[0] * inv_cols;
+    c.center(mean, v);
+  }
+  float s[1] = {dot(v, v)};
+  team_sum<1>(t, sh_sq, parity, s);
+  rstd = rsqrtf(__fmaf_rn(s[0], inv_cols, eps));
+}
+
+// v <- v * f (+ b)
+template <bool kAdd>
+__device__ __forceinline__ void scale_by(uint64_t (&v)[kElems / 2], const ParamSlot& f, const ParamSlot& b) {
+#pragma unroll
+  for (int k = 0; k < kElems / 4; ++k) {
+    uint64_t f0, f1;
+    f.pair(k, f0, f1);
+    if constexpr (kAdd) {
+      uint64_t b0, b1;
+      b.pair(k, b0, b1);
+      v[2 * k] = fma2(v[2 * k], f0, b0);
+      v[2 * k + 1] = fma2(v[2 * k + 1], f1, b1);
+    } else {
+      v[2 * k] = mul2(v[2 * k], f0);
+      v[2 * k + 1] = mul2(v[2 * k + 1], f1);
+    }
+  }
+}
+
+#ifndef KSMEM
+#define KSMEM 440
+#endif
+// Stages of the ring: up to three while 512 threads an SM (what the registers
+// allow) still fit its shared memory.
+constexpr int kParamBytes = kElems * 4, kThreadBytes = KSMEM;
+constexpr int ring_stages(int stage_bytes, int param_bytes) {
+  return 3 * stage_bytes + param_bytes <= kThreadBytes ? 3 : 2 * stage_bytes + param_bytes <= kThreadBytes ? 2 : 1;
+}
+template <int T, bool kAnywhere, bool kFull>
+struct Forward {
+  static constexpr int kStage = 2 * Ring<T, kAnywhere>::kWords * 16, kParams = (kFull ? 4 : 2) * kParamBytes;
+  static constexpr int kStages = ring_stages(kStage, kParams), kBytes = kStages * kStage + kParams;
+};
+template <int T, bool kAnywhere>
+struct Grad {
+  static constexpr int kStage = 4 * Ring<T, kAnywhere>::kWords * 16, kParams = 2 * kParamBytes;
+  static constexpr int kStages = ring_stages(kStage, kParams), kBytes = kStages * kStage + kParams;
+};
+// f32 rows that start anywhere need more than 512 threads' share: 256 threads.
+constexpr int norm_threads(int type) { return type == kF32 ? 256 : kTeamThreads; }
+
+// kFull: layer norms or biases too; a plain rms norm drops that code.
+template <int T, bool kAnywhere, bool kFull, bool kDrop>
+__global__ void __launch_bounds__(norm_threads(T)) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int P = kElems / 2, S = Forward<T, kAnywhere, kFull>::kStages, kWords = Ring<T, kAnywhere>::kWords;
+  extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<1> sh[4];
-  const bool warp_teams = a.shape.warp_teams;
-  const Team t = team_of(warp_teams);
-  const uint32_t teams = warp_teams ? blockDim.x >> 5 : 1;
-  uint64_t row = warp_teams ? uint64_t(blockIdx.x) * teams + (threadIdx.x >> 5) : blockIdx.x / t.ctas;
-  const uint64_t step = warp_teams ? uint64_t(gridDim.x) * teams : gridDim.x / t.ctas;
-  auto column = [&](int q) { return ((t.rank * Q + q) * t.threads + t.tid) * uint32_t(V); };
-  auto valid = [&](int q) { return column(q) < a.cols; };
+  const Team t = team_of(a.shape.warp_teams);
+  const Columns<T, kAnywhere> col(t, a);
+  const uint32_t teams = blockDim.x / t.threads;
+  // rows of a warp's teams follow one another: a warp goes on while its first has a row
+  const uint32_t team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
+  const uint64_t step = a.shape.warp_teams ? uint64_t(gridDim.x) * teams : gridDim.x / t.ctas;
+  uint64_t row = a.shape.warp_teams ? uint64_t(blockIdx.x) * teams + team : blockIdx.x / t.ctas;
+  const uint32_t ahead = a.shape.warp_teams ? t.lane / t.lanes : 0;  // rows this team is ahead of its warp's first
   const float inv_cols = 1.0f / float(a.cols);
+  const bool factor_on = a.post || a.gated || kDrop;
+  const uint32_t pitch = col.pitch, ring = shared_address(dynamic) + threadIdx.x * 16;
+  const uint32_t array = uint32_t(kWords) * pitch, stage_bytes = 2 * array, params = ring + S * stage_bytes;
+  const ParamSlot pre{params, pitch}, fac{params + kElems / 4 * pitch, pitch}, pre_b{params + 2 * (kElems / 4) * pitch, pitch},
+      fac_b{params + 3 * (kElems / 4) * pitch, pitch};
+  const uint64_t bytes = a.rows * a.cols * uint64_t(dtype_bytes(T)), advance = step * a.cols * uint64_t(dtype_bytes(T));
   pdl_enter();
   team_start(t);
-  const DropRun run = drop_run(a.drop, a.seed);
-  ActRaw<T, V> rx[Q], ry[Q];
-  auto fetch = [&](uint64_t r) {
+  DropRun run{};
+  if constexpr (kDrop) run = drop_run(a.drop, a.seed);
+  uint64_t next_row = row, next = col.offset(row);  // to be fetched
+  auto fetch = [&](uint32_t slot) {
+    if (next_row < a.rows) {
+      col.fetch(a.x, next, bytes, slot);
+      if (a.branch) col.fetch(a.y, next, bytes, slot + array);
+    }
+    copy_async_commit();
+    next_row += step;
+    next += advance;
+  };
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      rx[q].zero();
-      ry[q].zero();
-      if (valid(q)) {
-        rx[q].load(a.x, r * a.cols + column(q));
-        if (a.branch) ry[q].load(a.y, r * a.cols + column(q));
+  for (int s = 0; s < S; ++s) {
+    col.clear(ring + s * stage_bytes);
+    col.clear(ring + s * stage_bytes + array);
+  }
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(ring + s * stage_bytes);
+  {
+    float f[kElems];
+    col.params(a.w_pre, a.ptype, 0, 1.0f, f);
+    pre.write(f);
+    if constexpr (kFull) {
+      col.params(a.b_pre, a.ptype, 0, 0.0f, f);
+      pre_b.write(f);
+    }
+  }
+  uint64_t group_end = 0;  // the factors in shared memory are those of the rows before it
+  uint32_t slot = ring, free_slot = ring + (S - 1) * stage_bytes;
+  uint64_t off = col.offset(row);
+  for (int parity = 0; row - ahead < a.rows; row += step, off += advance, parity ^= 1) {
+    const bool on = row < a.rows;
+    fetch(free_slot);
+    if (a.branch && on && row >= group_end) {
+      // post weight, gate and the dropout's scale as one factor
+      const uint64_t group = row / a.rows_per_group;
+      group_end = (group + 1) * a.rows_per_group;
+      float g[kElems], f[kElems];
+      col.params(a.gate, a.ptype, group * a.cols, 1.0f, g);
+      col.params(a.w_post, a.ptype, 0, 1.0f, f);
+      const float scale = kDrop ? run.scale : 1.0f;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        g[e] *= scale;
+        f[e] *= g[e];
+      }
+      fac.write(f);
+      if constexpr (kFull) {
+        col.params(a.b_post, a.ptype, 0, 0.0f, f);
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) f[e] *= g[e];
+        fac_b.write(f);
       }
     }
-  };
-  if (row < a.rows) fetch(row);
-  for (int parity = 0; row < a.rows; row += step, parity ^= 1) {
-    float h[E], n[E];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      rx[q].widen(h + q * V);
-      ry[q].widen(n + q * V);
-    }
-    if (row + step < a.rows) fetch(row + step);
-    const bool writer = t.tid == 0 && t.rank == 0;
+    copy_async_wait<S - 1>();
+    uint64_t h[P];
+    const bool writer = on && t.tid == 0 && t.rank == 0;
     if (a.branch) {
+      uint64_t n[P];
+      col.read(slot + array, a.y, off, n);
       if (a.post) {
         float mean, rstd;
-        row_stats<E, V>(t, sh[0], sh[1], parity, a.layer, inv_cols, a.eps, n, valid, mean, rstd);
+        row_stats(t, col, sh[0], sh[1], parity, kFull && a.layer, inv_cols, a.eps, n, mean, rstd);
         if (writer) {
-          if (a.layer) a.stats_post[2 * row] = mean;
-          a.stats_post[a.layer ? 2 * row + 1 : row] = rstd;
+          if (kFull && a.layer) a.stats_post[2 * row] = mean;
+          a.stats_post[kFull && a.layer ? 2 * row + 1 : row] = rstd;
         }
+        const uint64_t r2 = both(rstd);
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          if (!valid(q)) continue;
-          float w[V];
-          param_load<V>(a.w_post, a.ptype, column(q), w);
-#pragma unroll
-          for (int j = 0; j < V; ++j) n[q * V + j] = (n[q * V + j] - mean) * rstd * w[j];
-          if (a.bias) {
-            param_load<V>(a.b_post, a.ptype, column(q), w);
-#pragma unroll
-            for (int j = 0; j < V; ++j) n[q * V + j] += w[j];
-          }
-        }
+        for (int k = 0; k < P; ++k) n[k] = mul2(n[k], r2);
       }
-      const uint64_t group = a.groups > 1 ? row / a.rows_per_group : 0;
+      if (factor_on) scale_by<kFull>(n, fac, fac_b);
+      if constexpr (kDrop) col.drop(run, off, n);
+      const uint64_t alpha = both(a.alpha);
+      col.read(slot, a.x, off, h);
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (!valid(q)) continue;
-        if (a.gated) {
-          float g[V];
-          param_load<V>(a.gate, a.ptype, group * a.cols + column(q), g);
-#pragma unroll
-          for (int j = 0; j < V; ++j) n[q * V + j] *= g[j];
-        }
-        if (a.drop.on) drop_unit<V>(run, row * a.cols + column(q), n + q * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[q * V + j] = __fmaf_rn(a.alpha, h[q * V + j], n[q * V + j]);
-        act_put<T, V>(a.h, row * a.cols + column(q), h + q * V);
-      }
+      for (int k = 0; k < P; ++k) h[k] = fma2(alpha, h[k], n[k]);
+      col.put(t, a.h, off, on, h);
+    } else {
+      col.read(slot, a.x, off, h);
     }
     if (a.pre) {
       float mean, rstd;
-      row_stats<E, V>(t, sh[2], sh[3], parity, a.layer, inv_cols, a.eps, h, valid, mean, rstd);
+      row_stats(t, col, sh[2], sh[3], parity, kFull && a.layer, inv_cols, a.eps, h, mean, rstd);
       if (writer) {
-        if (a.layer) a.stats_pre[2 * row] = mean;
-        a.stats_pre[a.layer ? 2 * row + 1 : row] = rstd;
+        if (kFull && a.layer) a.stats_pre[2 * row] = mean;
+        a.stats_pre[kFull && a.layer ? 2 * row + 1 : row] = rstd;
       }
+      const uint64_t r2 = both(rstd);
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (!valid(q)) continue;
-        float w[V], u[V];
-        param_load<V>(a.w_pre, a.ptype, column(q), w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[j] = (h[q * V + j] - mean) * rstd * w[j];
-        if (a.bias) {
-          param_load<V>(a.b_pre, a.ptype, column(q), w);
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[j] += w[j];
-        }
-        act_put<T, V>(a.u, row * a.cols + column(q), u);
-      }
+      for (int k = 0; k < P; ++k) h[k] = mul2(h[k], r2);
+      scale_by<kFull>(h, pre, pre_b);
+      col.put(t, a.u, off, on, h);
     }
+    free_slot = slot;  // read by its own thread alone, and that is done
+    slot = slot == ring + (S - 1) * stage_bytes ? ring : slot + stage_bytes;
   }
 }
 
 // A team takes a chunk of one group's rows and leaves its column sums in
 // a.partial, [kind][group * chunks + chunk][cols].
-template <int T, int V, int E, bool kBias>
-__global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const NormArgs a, const NormSums kinds) {
-  constexpr int Q = E / V;
-  __shared__ TeamRecords<2> sh[2];
-  __shared__ float joined[32 * E];
-  const bool warp_teams = a.shape.warp_teams;
-  const Team t = team_of(warp_teams);
-  const uint32_t teams = warp_teams ? blockDim.x >> 5 : 1, team = warp_teams ? threadIdx.x >> 5 : 0;
+template <int T, bool kAnywhere, bool kFull, bool kDrop>
+__global__ void __launch_bounds__(norm_threads(T)) norm_grad_kernel(const __grid_constant__ NormArgs a, const NormSums kinds) {
+  constexpr int E = kElems, P = E / 2, V = act_vec<T>(), Q = E / V, S = Grad<T, kAnywhere>::kStages,
+                kWords = Ring<T, kAnywhere>::kWords, N = kFull ? 2 : 1;
+  extern __shared__ uint4 dynamic[];
+  __shared__ TeamRecords<N> sh[2];
+  const Team t = team_of(a.shape.warp_teams);
+  const Columns<T, kAnywhere> col(t, a);
+  const uint32_t teams = a.shape.warp_teams ? blockDim.x / t.threads : 1, team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
+  const uint32_t ahead = a.shape.warp_teams ? t.lane / t.lanes : 0;
   const uint32_t place = blockIdx.x / t.ctas;  // this CTA's (or cluster's) chunk among all
   const uint32_t group = place / a.chunks, chunk = place % a.chunks;
   const uint64_t begin = uint64_t(group) * a.rows_per_group + a.rows_per_group * chunk / a.chunks;
   const uint64_t end = uint64_t(group) * a.rows_per_group + a.rows_per_group * (chunk + 1) / a.chunks;
-  auto column = [&](int q) { return ((t.rank * Q + q) * t.threads + t.tid) * uint32_t(V); };
-  auto valid = [&](int q) { return column(q) < a.cols; };
   const float inv_cols = 1.0f / float(a.cols);
   const bool need_y = a.branch && (a.post || a.gated);
+  const uint32_t pitch = col.pitch, ring = shared_address(dynamic) + threadIdx.x * 16;
+  const uint32_t array = uint32_t(kWords) * pitch, stage_bytes = 4 * array, params = ring + S * stage_bytes;
+  const ParamSlot pre{params, pitch}, fac{params + E / 4 * pitch, pitch};
+  const uint64_t bytes = a.rows * a.cols * uint64_t(dtype_bytes(T)), advance = teams * uint64_t(a.cols) * dtype_bytes(T);
   pdl_enter();
   team_start(t);
-  const DropRun run = drop_run(a.drop, a.seed);
-  float acc_t[E] = {}, acc_p[E] = {}, acc_s[kBias ? E : 1] = {}, acc_q[kBias ? E : 1] = {};
-  ActRaw<T, V> rdh[Q], rdu[Q], rh[Q], ry[Q];
-  float mean_h = 0.0f, rstd_h = 0.0f, mean_y = 0.0f, rstd_y = 1.0f;
-  auto fetch = [&](uint64_t r) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      rdh[q].zero(); rdu[q].zero(); rh[q].zero(); ry[q].zero();
-      if (!valid(q)) continue;
-      const uint64_t at = r * a.cols + column(q);
-      if (a.branch) rdh[q].load(a.dh, at);
+  DropRun run{};
+  if constexpr (kDrop) run = drop_run(a.drop, a.seed);
+  uint64_t row = begin + team, next_row = row, next = col.offset(row), off = next;
+  auto fetch = [&](uint32_t slot) {
+    if (next_row < end) {
+      if (a.branch) col.fetch(a.dh, next, bytes, slot);
       if (a.pre) {
-        rdu[q].load(a.du, at);
-        rh[q].load(a.h_in, at);
+        col.fetch(a.du, next, bytes, slot + array);
+        col.fetch(a.h_in, next, bytes, slot + 2 * array);
       }
-      if (need_y) ry[q].load(a.y, at);
+      if (need_y) col.fetch(a.y, next, bytes, slot + 3 * array);
     }
-    if (a.pre) {
-      if (a.layer) mean_h = __ldg(a.stats_pre_in + 2 * r);
-      rstd_h = __ldg(a.stats_pre_in + (a.layer ? 2 * r + 1 : r));
-    }
-    if (a.post) {
-      if (a.layer) mean_y = __ldg(a.stats_post_in + 2 * r);
-      rstd_y = __ldg(a.stats_post_in + (a.layer ? 2 * r + 1 : r));
-    }
+    copy_async_commit();
+    next_row += teams;
+    next += advance;
   };
-  uint64_t row = begin + team;
-  if (row < end) fetch(row);
-  for (int parity = 0; row < end; row += teams, parity ^= 1) {
-    float g[E], du[E], hh[E], yy[E];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      rdh[q].widen(g + q * V);
-      rdu[q].widen(du + q * V);
-      rh[q].widen(hh + q * V);
-      ry[q].widen(yy + q * V);
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) col.clear(ring + s * stage_bytes + k * array);
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(ring + s * stage_bytes);
+  // post weight, gate and dropout scale as one factor; the scale of the sums
+  // over dropped gradients is applied once, to the sums
+  const float scale = kDrop ? run.scale : 1.0f;
+  {
+    float f[E], g[E];
+    col.params(a.w_pre, a.ptype, 0, 1.0f, f);
+    pre.write(f);
+    col.params(a.w_post, a.ptype, 0, 1.0f, f);
+    col.params(a.gate, a.ptype, uint64_t(group) * a.cols, 1.0f, g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= g[e] * scale;
+    fac.write(f);
+  }
+  uint64_t acc_t[P] = {}, acc_p[P] = {}, acc_s[kFull ? P : 1] = {}, acc_q[kFull ? P : 1] = {};
+  uint32_t slot = ring, free_slot = ring + (S - 1) * stage_bytes;
+  for (int parity = 0; row - ahead < end; row += teams, off += advance, parity ^= 1) {
+    const bool on = row < end;  // a row that is not there counts as zeros
+    float mean_h = 0.0f, rstd_h = 0.0f, mean_y = 0.0f, rstd_y = 0.0f;
+    if (a.pre && on) {
+      if (kFull && a.layer) mean_h = __ldg(a.stats_pre_in + 2 * row);
+      rstd_h = __ldg(a.stats_pre_in + (kFull && a.layer ? 2 * row + 1 : row));
     }
-    const float mh = mean_h, sh_ = rstd_h, my = mean_y, sy = rstd_y;
-    if (row + teams < end) fetch(row + teams);
+    if (a.post && on) {
+      if (kFull && a.layer) mean_y = __ldg(a.stats_post_in + 2 * row);
+      rstd_y = __ldg(a.stats_post_in + (kFull && a.layer ? 2 * row + 1 : row));
+    }
+    fetch(free_slot);
+    copy_async_wait<S - 1>();
+    uint64_t g[P] = {};
     if (a.pre) {
-      float s[2] = {0.0f, 0.0f};
+      uint64_t du[P], hh[P];
+      col.read(slot + array, a.du, off, du);
+      col.read(slot + 2 * array, a.h_in, off, hh);
+      if (!on) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (!valid(q)) continue;
-        float w[V];
-        param_load<V>(a.w_pre, a.ptype, column(q), w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int e = q * V + j;
-          hh[e] = (hh[e] - mh) * sh_;
-          acc_p[e] = __fmaf_rn(du[e], hh[e], acc_p[e]);
-          if constexpr (kBias) acc_q[e] += du[e];
-          du[e] *= w[j];
-          s[0] = __fmaf_rn(du[e], hh[e], s[0]);
-          s[1] += du[e];
-        }
+        for (int k = 0; k < P; ++k) du[k] = hh[k] = 0;
       }
-      team_sum<2>(t, sh[0], parity, s);
-      const float k = s[0] * inv_cols, m = a.layer ? s[1] * inv_cols : 0.0f;
+      if (kFull && a.layer) col.center(mean_h, hh);
+      const uint64_t r2 = both(rstd_h);
 #pragma unroll
-      for (int e = 0; e < E; ++e) g[e] = __fmaf_rn(sh_, du[e] - m - hh[e] * k, g[e]);
+      for (int k = 0; k < P; ++k) {
+        hh[k] = mul2(hh[k], r2);
+        acc_p[k] = fma2(du[k], hh[k], acc_p[k]);
+        if constexpr (kFull) acc_q[k] = add2(acc_q[k], du[k]);
+      }
+      scale_by<false>(du, pre, pre);
+      float s[N];
+      s[0] = dot(du, hh);
+      if constexpr (kFull) s[1] = a.layer ? total(du) : 0.0f;
+      team_sum<N>(t, sh[0], parity, s);
+      const uint64_t k2 = both(-s[0] * inv_cols);
+      if (a.branch) col.read(slot, a.dh, off, g);
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        uint64_t v = fma2(hh[k], k2, du[k]);
+        if constexpr (kFull) v = add2(v, both(-s[1] * inv_cols));
+        g[k] = fma2(r2, v, g[k]);
+      }
+    } else if (a.branch) {
+      col.read(slot, a.dh, off, g);
     }
+    if (!on) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      if (!valid(q)) continue;
-      float o[V];
+      for (int k = 0; k < P; ++k) g[k] = 0;
+    }
+    {
+      const uint64_t alpha = both(a.alpha);
+      uint64_t o[P];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = a.alpha * g[q * V + j];
-      act_put<T, V>(a.dx, row * a.cols + column(q), o);
+      for (int k = 0; k < P; ++k) o[k] = mul2(alpha, g[k]);
+      col.put(t, a.dx, off, on, o);
     }
     if (a.branch) {
-      float s[2] = {0.0f, 0.0f};
+      if constexpr (kDrop) col.drop(run, off, g);
+      uint64_t yy[P] = {};
+      if (need_y) {
+        col.read(slot + 3 * array, a.y, off, yy);
+        if (!on) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (!valid(q)) continue;
-        if (a.drop.on) drop_unit<V>(run, row * a.cols + column(q), g + q * V);
-        float gate[V], w[V];
-        if (a.gated) param_load<V>(a.gate, a.ptype, uint64_t(group) * a.cols + column(q), gate);
-        if (a.post) param_load<V>(a.w_post, a.ptype, column(q), w);
+          for (int k = 0; k < P; ++k) yy[k] = 0;
+        }
+        if (a.post) {
+          if (kFull && a.layer) col.center(mean_y, yy);
+          const uint64_t r2 = both(rstd_y);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int e = q * V + j;
-          if (a.post) yy[e] = (yy[e] - my) * sy;
-          acc_t[e] = __fmaf_rn(g[e], yy[e], acc_t[e]);
-          if constexpr (kBias) acc_s[e] += g[e];
-          if (a.gated) g[e] *= gate[j];
-          if (a.post) {
-            g[e] *= w[j];
-            s[0] = __fmaf_rn(g[e], yy[e], s[0]);
-            s[1] += g[e];
-          }
+          for (int k = 0; k < P; ++k) yy[k] = mul2(yy[k], r2);
+        }
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          acc_t[k] = fma2(g[k], yy[k], acc_t[k]);
+          if constexpr (kFull) acc_s[k] = add2(acc_s[k], g[k]);
         }
       }
+      scale_by<false>(g, fac, fac);
       if (a.post) {
-        team_sum<2>(t, sh[1], parity, s);
-        const float k = s[0] * inv_cols, m = a.layer ? s[1] * inv_cols : 0.0f;
+        float s[N];
+        s[0] = dot(g, yy);
+        if constexpr (kFull) s[1] = a.layer ? total(g) : 0.0f;
+        team_sum<N>(t, sh[1], parity, s);
+        const uint64_t r2 = both(rstd_y), k2 = both(-s[0] * inv_cols);
 #pragma unroll
-        for (int e = 0; e < E; ++e) g[e] = sy * (g[e] - m - yy[e] * k);
-      }
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (valid(q)) act_put<T, V>(a.dy, row * a.cols + column(q), g + q * V);
-    }
-  }
-  // the team's column sums; warps of a CTA that were teams of their own are
-  // added in warp order
-  const uint64_t places = uint64_t(a.groups) * a.chunks;
-  auto put = [&](const float* v, int kind) {
-    float* out = a.partial + (uint64_t(kind) * places + place) * a.cols;
-    if (!warp_teams) {
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (valid(q)) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) out[column(q) + j] = v[q * V + j];
+        for (int k = 0; k < P; ++k) {
+          uint64_t v = fma2(yy[k], k2, g[k]);
+          if constexpr (kFull) v = add2(v, both(-s[1] * inv_cols));
+          g[k] = mul2(r2, v);
         }
+      }
+      col.put(t, a.dy, off, on, g);
+    }
+    free_slot = slot;
+    slot = slot == ring + (S - 1) * stage_bytes ? ring : slot + stage_bytes;
+  }
+  // the team's column sums; teams that share a CTA are added in their order,
+  // through shared memory (the ring is done with)
+  const uint64_t places = uint64_t(a.groups) * a.chunks;
+  float* const joined = reinterpret_cast<float*>(dynamic);
+  copy_async_wait<0>();
+  __syncthreads();
+  auto put = [&](const uint64_t (&pairs)[P], float by, int kind) {
+    float v[E];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      unpack2(pairs[k], v[2 * k], v[2 * k + 1]);
+      v[2 * k] *= by;
+      v[2 * k + 1] *= by;
+    }
+    float* out = a.partial + (uint64_t(kind) * places + place) * a.cols;
+    if (!a.shape.warp_teams) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < col.count(q)) out[col.at(q) + j] = v[q * V + j];
       return;
     }
     for (uint32_t w = 0; w < teams; ++w) {
       if (team == w) {
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-          if (valid(q)) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              float* at = joined + column(q) + j;
+          for (int j = 0; j < V; ++j)
+            if (j < col.count(q)) {
+              float* at = joined + col.at(q) + j;
               *at = w ? *at + v[q * V + j] : v[q * V + j];
             }
-          }
       }
       __syncthreads();
     }
@@ -318,13 +612,13 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const NormArgs 
     __syncthreads();
   };
   int kind = 0;
-  if (kinds.t) put(acc_t, kind++);
-  if constexpr (kBias) {
-    if (kinds.s) put(acc_s, kind++);
+  if (kinds.t) put(acc_t, scale, kind++);
+  if constexpr (kFull) {
+    if (kinds.s) put(acc_s, scale, kind++);
   }
-  if (kinds.p) put(acc_p, kind++);
-  if constexpr (kBias) {
-    if (kinds.q) put(acc_q, kind++);
+  if (kinds.p) put(acc_p, 1.0f, kind++);
+  if constexpr (kFull) {
+    if (kinds.q) put(acc_q, 1.0f, kind++);
   }
 }
 
@@ -413,38 +707,46 @@ __global__ void __launch_bounds__(32 * kJoinWarps) norm_grad_join_kernel(const N
   }
 }
 
-template <int T, int V>
-const void* forward_kernel(int elems) {
-  return elems == 8 ? (const void*)norm_rows_kernel<T, V, 8> : (const void*)norm_rows_kernel<T, V, 16>;
+struct Chosen {
+  const void* kernel;
+  unsigned shared_bytes;
+};
+template <int T, bool kAnywhere, bool kFull, bool kDrop>
+Chosen choice(const NormArgs& a, bool grad) {
+  const unsigned threads = unsigned(a.shape.threads);
+  if (grad) return {(const void*)norm_grad_kernel<T, kAnywhere, kFull, kDrop>, threads * unsigned(Grad<T, kAnywhere>::kBytes)};
+  return {(const void*)norm_rows_kernel<T, kAnywhere, kFull, kDrop>, threads * unsigned(Forward<T, kAnywhere, kFull>::kBytes)};
 }
-template <int T, int V>
-const void* grad_kernel(bool bias) {
-  return bias ? (const void*)norm_grad_kernel<T, V, 8, true> : (const void*)norm_grad_kernel<T, V, 8, false>;
+template <int T, bool kAnywhere>
+Chosen choice_of_switches(const NormArgs& a, bool grad) {
+  if (a.layer || a.bias)
+    return a.drop.on ? choice<T, kAnywhere, true, true>(a, grad) : choice<T, kAnywhere, true, false>(a, grad);
+  return a.drop.on ? choice<T, kAnywhere, false, true>(a, grad) : choice<T, kAnywhere, false, false>(a, grad);
 }
 template <int T>
-const void* kernel_of_type(const NormArgs& a, bool grad, bool vec) {
-  constexpr int V = act_vec<T>();
-  if (grad) return vec ? grad_kernel<T, V>(a.bias) : grad_kernel<T, 1>(a.bias);
-  return vec ? forward_kernel<T, V>(a.shape.elems) : forward_kernel<T, 1>(a.shape.elems);
+Chosen choice_of_type(const NormArgs& a, bool grad, bool aligned) {
+  return aligned ? choice_of_switches<T, false>(a, grad) : choice_of_switches<T, true>(a, grad);
 }
-const void* kernel_for(const NormArgs& a, bool grad, bool vec) {
-  return a.type == kF32 ? kernel_of_type<kF32>(a, grad, vec)
-         : a.type == kF16 ? kernel_of_type<kF16>(a, grad, vec) : kernel_of_type<kBF16>(a, grad, vec);
+// The kernel of a step, its shared memory allowed (above 48 KB that has to be asked for).
+cudaError_t choose(const NormArgs& a, bool grad, bool aligned, Chosen* c) {
+  *c = a.type == kF32   ? choice_of_type<kF32>(a, grad, aligned)
+       : a.type == kF16 ? choice_of_type<kF16>(a, grad, aligned) : choice_of_type<kBF16>(a, grad, aligned);
+  return c->shared_bytes <= 32 * 1024
+             ? cudaSuccess
+             : cudaFuncSetAttribute(c->kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(c->shared_bytes));
 }
 
 }  // namespace
 
-TeamShape norm_shape(uint64_t cols, bool grad) {
-  // The gradient keeps column sums beside four rows: 8 elements a thread, and
-  // a cluster for rows beyond 4096 columns (16 elements spilled).
-  TeamShape s{0, kWarpTeamThreads, 1, 8};
-  if (!grad && cols > 32 * 8) s.elems = cols <= 32 * 16 ? 16 : cols <= 8 * kTeamThreads ? 8 : 16;
-  if (cols <= uint64_t(32) * s.elems) {
-    s.warp_teams = 1;
+TeamShape norm_shape(uint64_t cols, int type) {
+  TeamShape s{0, kWarpTeamThreads, 1, kElems};
+  if (cols <= 32 * kElems) {
+    s.warp_teams = 4;
+    while (cols > uint64_t(s.warp_teams) * kElems) s.warp_teams *= 2;
     return s;
   }
-  while (cols > uint64_t(kTeamThreads) * s.elems * s.ctas) s.ctas *= 2;
-  const uint64_t per = uint64_t(s.elems) * s.ctas;
+  while (cols > uint64_t(norm_threads(type)) * kElems * s.ctas) s.ctas *= 2;
+  const uint64_t per = uint64_t(kElems) * s.ctas;
   s.threads = int((((cols + per - 1) / per) + 31) / 32 * 32);
   return s;
 }
@@ -454,25 +756,31 @@ NormSums norm_sums(const NormArgs& a) {
 }
 
 cudaError_t norm_occupancy(const NormArgs& a, bool grad, int* blocks_per_sm) {
-  const uint64_t vec = a.type == kF32 ? 4 : 8;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, kernel_for(a, grad, a.cols % vec == 0),
-                                                       a.shape.threads, 0);
+  Chosen c;
+  const cudaError_t e = choose(a, grad, a.cols % (a.type == kF32 ? 4 : 8) == 0, &c);
+  if (e != cudaSuccess) return e;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);
 }
 
-cudaError_t norm_launch(const NormArgs& a, bool vec, int grid, cudaStream_t stream) {
+cudaError_t norm_launch(const NormArgs& a, bool aligned, int grid, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
+  Chosen c;
+  const cudaError_t e = choose(a, false, aligned, &c);
+  if (e != cudaSuccess) return e;
   NormArgs args = a;
   void* params[] = {&args};
-  return launch_rows(kernel_for(a, false, vec), a.shape, unsigned(grid), 0, params, stream);
+  return launch_rows(c.kernel, a.shape, unsigned(grid), c.shared_bytes, params, stream);
 }
 
-cudaError_t norm_grad_launch(const NormArgs& a, bool vec, cudaStream_t stream) {
+cudaError_t norm_grad_launch(const NormArgs& a, bool aligned, cudaStream_t stream) {
   NormArgs args = a;
   NormSums kinds = norm_sums(a);
   if (a.rows) {
+    Chosen c;
+    cudaError_t e = choose(a, true, aligned, &c);
+    if (e != cudaSuccess) return e;
     void* params[] = {&args, &kinds};
-    const cudaError_t e = launch_rows(kernel_for(a, true, vec), a.shape,
-                                      a.groups * a.chunks * unsigned(a.shape.ctas), 0, params, stream);
+    e = launch_rows(c.kernel, a.shape, a.groups * a.chunks * unsigned(a.shape.ctas), c.shared_bytes, params, stream);
     if (e != cudaSuccess) return e;
   } else {
     args.chunks = 0;  // the column sums of no rows are zero

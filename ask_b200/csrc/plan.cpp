@@ -1011,13 +1011,13 @@ void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
   }
   in(a.drop.on, kI64, 2);
 
-  a.shape = norm_shape(cols, grad);
+  a.shape = norm_shape(cols, a.type);
   pl.block = a.shape.threads;
   int occ = 2;
   if (pl.device >= 0) check_cuda(norm_occupancy(a, grad, &occ), "occupancy");
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
-  const uint64_t teams = a.shape.warp_teams ? uint64_t(a.shape.threads) / 32 : 1;
+  const uint64_t teams = uint64_t(team_count(a.shape));
   const std::string name = std::string(a.layer ? "layer_" : "rms_") + kTypeNames[a.type];
   if (!grad) {
     pl.kernel = "norm_rows_" + name;
@@ -1101,7 +1101,7 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
   if (pl.device >= 0) check_cuda(bias_softmax_occupancy(a, grad, &occ), "occupancy");
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
-  const uint64_t teams = a.shape.warp_teams ? uint64_t(a.shape.threads) / 32 : 1;
+  const uint64_t teams = uint64_t(team_count(a.shape));
   const uint64_t pairs = mul_checked(a.batch, a.queries);
   a.chunks = heads ? uint32_t(chunk_count(heads, (pairs + teams - 1) / teams, slots)) : 1;
   const uint64_t ctas = mul_checked(mul_checked(heads, a.chunks), uint64_t(a.shape.ctas));

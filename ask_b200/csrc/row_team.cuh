@@ -1,8 +1,9 @@
 // The threads that share a row, and their reductions.
 //
-// A row is held by a warp (short rows: several independent teams in a CTA, no
-// barrier), by a CTA, or by a cluster of up to eight CTAs (rows longer than a
-// CTA's registers hold, or so few rows that most SMs would idle).  A reduction
+// A row is held by part of a warp or a warp (short rows: several independent
+// teams in a CTA, no barrier), by a CTA, or by a cluster of up to eight CTAs
+// (rows longer than a CTA's registers hold, or so few rows that most SMs would
+// idle).  A reduction
 // folds each warp by shuffles, then every warp writes its record into the
 // shared memory of every CTA of the team (distributed shared memory within a
 // cluster), one barrier follows, and every thread folds the records in warp
@@ -29,6 +30,7 @@ constexpr int kTeamRecords = kTeamThreads / 32 * kTeamCluster;
 struct Team {
   uint32_t tid;      // thread within this CTA's part of the team
   uint32_t threads;  // threads of that part
+  uint32_t lanes;    // lanes of a warp that belong to one team
   uint32_t lane, warp, warps;
   uint32_t ctas, rank;  // CTAs of the team (the cluster) and this one's place among them
 };
@@ -54,13 +56,15 @@ __device__ __forceinline__ uint32_t peer_address(const void* mine, uint32_t rank
   return r;
 }
 
-// `warp_teams`: every warp is a team of its own.
-__device__ __forceinline__ Team team_of(bool warp_teams) {
+// `warp_teams`: the lanes of a team within a warp (4 to 32, a power of two), or
+// 0 where the CTA or the cluster is the team.
+__device__ __forceinline__ Team team_of(int warp_teams) {
   Team t;
   t.lane = threadIdx.x & 31u;
+  t.lanes = warp_teams ? uint32_t(warp_teams) : 32u;
   if (warp_teams) {
-    t.tid = t.lane;
-    t.threads = 32;
+    t.tid = t.lane & (t.lanes - 1);
+    t.threads = t.lanes;
     t.warp = 0;
     t.warps = 1;
     t.ctas = 1;
@@ -83,7 +87,7 @@ __device__ __forceinline__ void team_start(const Team& t) {
 }
 
 template <int N>
-struct TeamRecords {
+struct alignas(16) TeamRecords {
   float v[2][kTeamRecords][N];
 };
 
@@ -112,13 +116,22 @@ template <int N>
 __device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int parity, float (&v)[N]) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
+    if (uint32_t(d) >= t.lanes) continue;
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], d);
   }
   const uint32_t records = t.warps * t.ctas;
   if (records == 1) return;
   team_exchange<N>(t, sh, parity, v);
-  if (records <= 8) {
+  if (records == 8) {  // rows of 4096: no loop
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float r[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] = sh.v[parity][k][n];
+      v[n] = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+    }
+  } else if (records < 8) {
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] = sh.v[parity][0][n];
     for (uint32_t k = 1; k < records; ++k) {
