@@ -129,6 +129,44 @@ __device__ __forceinline__ void act_put(void* p, uint64_t i, const float* v) {
   st_stream_v4(static_cast<char*>(p) + i * dtype_bytes(T), act_narrow<T>(v));
 }
 
+// Shared memory by its 32-bit address, and asynchronous 16-byte copies into it.
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void copy_to_shared(uint32_t at, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+}
+
+// f32 pairs.
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+__device__ __forceinline__ float sum2(uint64_t v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return lo + hi;
+}
+template <int T>
+__device__ __forceinline__ void act_widen2(const uint4& r, uint64_t* v) {
+  float f[act_vec<T>()];
+  act_widen<T>(r, f);
+#pragma unroll
+  for (int k = 0; k < act_vec<T>() / 2; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
+}
+template <int T>
+__device__ __forceinline__ uint4 act_narrow2(const uint64_t* v) {
+  float f[act_vec<T>()];
+#pragma unroll
+  for (int k = 0; k < act_vec<T>() / 2; ++k) unpack2(v[k], f[2 * k], f[2 * k + 1]);
+  return act_narrow<T>(f);
+}
+
 // V parameters (weights, gates) of run-time type starting at column c: read
 // again for every row, so they stay in L1 or L2.
 template <int V>

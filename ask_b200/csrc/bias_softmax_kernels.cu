@@ -21,14 +21,17 @@
 // Rows start anywhere (any number of keys): a row is read and written in the
 // tensor's own aligned 16-byte units, whose first and last may hold elements of
 // the neighbouring rows; those are masked, and only such cut units are stored
-// element by element.  Units without a visible key are not read.
+// element by element.  Units without a visible key are not read.  The next row's
+// units are on their way (cp.async into words that only their own thread reads)
+// while this row is worked on.
 //
 // exp(l - m) is 2^(l L - RN(m L)) with L = log2 e: an element costs a fused
-// multiply-add for its logit, one for the exponent and ex2.approx (relative
-// error 2^-22).  The rounding of m L is one factor for all that share m.
-// Where m L could overflow (|m| > 2^100: rows at the type's lowest value) the
-// difference is taken first.  Each warp takes its own maximum, and its sum is
-// rescaled when the team's records meet: one exchange a row.
+// multiply-add for its logit, one for the exponent (both on f32 pairs) and
+// ex2.approx (relative error 2^-22).  The rounding of m L is one factor for all
+// that share m.  Where m L could overflow (|m| > 2^100: rows at the type's
+// lowest value) the difference is taken first.  Each warp takes its own
+// maximum, and its sum is rescaled when the team's records meet: one exchange a
+// row.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -43,17 +46,44 @@ namespace askb {
 
 namespace {
 
-constexpr int kWarpTeamThreads = 256;
+#ifndef KWT
+#define KWT 128
+#endif
+constexpr int kWarpTeamThreads = KWT;
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// The window's geometry: distances rel in [-W, hi] at index rel + W.
+// The window's geometry: distances rel in [-W, hi], and V - 1 places beyond
+// either end, so that a unit that reaches into the window has a place for each
+// of its elements.  Place i lies at word i + i / V: the lanes of a warp, whose
+// units are V places apart, then fall on different banks.
+template <int V>
 struct Window {
-  int w, hi, size;
+  int w, hi;
+  __host__ __device__ explicit Window(const BiasSoftmaxArgs& a)
+      : w(a.n_thresholds ? a.thresholds[a.n_thresholds - 1] : 0), hi(a.bidirectional ? w : 0) {}
+  __host__ __device__ int places() const { return w + hi + 1 + 2 * (V - 1); }
+  __host__ __device__ static int word(int place) { return place + place / V; }
+  __host__ __device__ int words() const { return word(places() - 1) + 1; }
+  __host__ __device__ int place(int rel) const { return rel + w + (V - 1); }
+  __host__ __device__ int rel(int place) const { return place - w - (V - 1); }
 };
-__host__ __device__ inline Window window_of(const BiasSoftmaxArgs& a) {
-  const int w = a.n_thresholds ? a.thresholds[a.n_thresholds - 1] : 0;
-  const int hi = a.bidirectional ? w : 0;
-  return Window{w, hi, w + hi + 1};
+// The words of V places from `place` on: word(place) + j, and one more from the
+// next multiple of V on.
+template <int V>
+struct Places {
+  uint32_t at;  // shared address of the first
+  int wrap;     // j from which one word is skipped
+  __device__ __forceinline__ Places(uint32_t base, int place)
+      : at(base + 4u * uint32_t(place + place / V)), wrap(V - place % V) {}
+  __device__ __forceinline__ uint32_t operator()(int j) const { return at + (j >= wrap ? 4u * j + 4u : 4u * j); }
+};
+__device__ __forceinline__ float ld_shared_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t at, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ int bucket_of(const BiasSoftmaxArgs& a, int rel) {
@@ -67,159 +97,262 @@ __device__ __forceinline__ int bucket_of(const BiasSoftmaxArgs& a, int rel) {
 }
 
 // The head's bias by distance.
-__device__ __forceinline__ void fill_window(const BiasSoftmaxArgs& a, const Window& win, uint32_t head, float* lut) {
-  for (int i = int(threadIdx.x); i < win.size; i += int(blockDim.x)) {
+template <int V>
+__device__ __forceinline__ void fill_window(const BiasSoftmaxArgs& a, const Window<V>& win, uint32_t head, float* lut) {
+  for (int i = int(threadIdx.x); i < win.places(); i += int(blockDim.x)) {
     float v[1];
-    param_load<1>(a.table, a.table_type, uint64_t(bucket_of(a, i - win.w)) * a.heads + head, v);
-    lut[i] = v[0];
+    param_load<1>(a.table, a.table_type, uint64_t(bucket_of(a, win.rel(i))) * a.heads + head, v);
+    lut[win.word(i)] = v[0];
   }
 }
 
-// One row as the team sees it.
-struct Row {
-  uint64_t index;      // of the row
-  uint64_t first;      // element index of its first unit
-  int shift;           // elements of that unit before the row
-  int pos, visible;    // query position; keys [0, visible) are seen
+// The rows of a team, one after the other: pairs (batch, query) of one head.
+template <int T>
+struct Rows {
+  static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
+  const BiasSoftmaxArgs& a;
+  uint32_t head, step, b, q;
+  uint64_t left;          // rows from this one on, in steps
+  int length, place;      // of the sequence: keys in use, position of its query 0
+  // of the row
+  uint64_t index, first;  // byte offset of its first unit
+  int shift;              // elements of that unit before the row
+  int pos, visible;       // query position; keys [0, visible) are seen
+
+  __device__ __forceinline__ Rows(const BiasSoftmaxArgs& args, const Team& t) : a(args) {
+    const uint32_t cta = blockIdx.x / t.ctas, chunk = cta / a.heads;
+    const uint64_t n = a.batch * a.queries, begin = n * chunk / a.chunks, end = n * (chunk + 1) / a.chunks;
+    const uint32_t team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
+    head = cta % a.heads;
+    step = a.shape.warp_teams ? blockDim.x / t.threads : 1;
+    left = begin + team < end ? (end - begin - team + step - 1) / step : 0;
+    b = uint32_t((begin + team) / a.queries);
+    q = uint32_t((begin + team) % a.queries);
+  }
+  __device__ __forceinline__ void sequence() {
+    length = int(a.keys);
+    place = 0;
+    if (a.lengths) length = max(min(__ldg(a.lengths + b), length), 0);
+    if (a.offsets) place = __ldg(a.offsets + b);
+  }
+  __device__ __forceinline__ void locate() {
+    index = (uint64_t(b) * a.heads + head) * a.queries + q;
+    const uint64_t e = index * a.keys;
+    shift = int(uint32_t(e) & uint32_t(V - 1));
+    first = (e - uint64_t(shift)) * B;
+    const int64_t at = int64_t(place) + int64_t(q);
+    visible = length;
+    if (a.causal) visible = int(max(min(int64_t(length), at + 1), int64_t(0)));
+    // far positions meet only the window's ends, whatever their distance
+    pos = int(max(min(at, int64_t(1) << 30), -(int64_t(1) << 30)));
+  }
+  // to be called once before the first row, then to go on
+  __device__ __forceinline__ void start() {
+    if (left) {
+      sequence();
+      locate();
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (--left == 0) return;
+    q += step;
+    if (q >= a.queries) {
+      const uint32_t n = q / uint32_t(a.queries);
+      b += n;
+      q -= n * uint32_t(a.queries);
+      sequence();
+    }
+    locate();
+  }
 };
-template <int V>
-__device__ __forceinline__ Row row_of(const BiasSoftmaxArgs& a, uint32_t head, uint64_t pair) {
-  Row r;
-  const uint64_t b = pair / a.queries, q = pair - b * a.queries;
-  r.index = (b * a.heads + head) * a.queries + q;
-  const uint64_t e = r.index * a.keys;
-  r.shift = int(e % uint64_t(V));
-  r.first = e - uint64_t(r.shift);
-  const int64_t pos = int64_t(q) + (a.offsets ? int64_t(__ldg(a.offsets + b)) : 0);
-  int64_t seen = a.keys;
-  if (a.lengths) seen = min(seen, int64_t(__ldg(a.lengths + b)));
-  if (a.causal) seen = min(seen, pos + 1);
-  r.visible = int(max(seen, int64_t(0)));
-  // far positions meet only the window's ends, whatever their distance
-  r.pos = int(max(min(pos, int64_t(1) << 30), -(int64_t(1) << 30)));
-  return r;
-}
 
-// The unit's elements of `p`, where any is visible.
-template <int T, int V>
-__device__ __forceinline__ void load_seen(const BiasSoftmaxArgs& a, const void* p, const Row& r, int k0, uint64_t total,
-                                          float* v) {
-  const uint64_t at = r.first + uint64_t(int64_t(k0) + r.shift);
-  if (k0 >= r.visible || k0 + V <= 0) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.0f;
-  } else if (a.aligned && at + V <= total) {
-    ActRaw<T, V> raw;
-    raw.load(p, at);
-    raw.widen(v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = k0 + j >= 0 && k0 + j < r.visible ? act_load<T>(p, at + j) : 0.0f;
-  }
-}
-// The unit's elements that belong to the row.
-template <int T, int V>
-__device__ __forceinline__ void store_row(const BiasSoftmaxArgs& a, const Row& r, int k0, const float* v) {
-  if (k0 >= int(a.keys)) return;
-  const uint64_t at = r.first + uint64_t(int64_t(k0) + r.shift);
-  if (a.aligned && k0 >= 0 && k0 + V <= int(a.keys)) {
-    act_put<T, V>(a.out, at, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (k0 + j >= 0 && k0 + j < int(a.keys)) act_store<T>(a.out, at + j, v[j]);
-  }
-}
+// One row of a team in flight or at work: which units the thread has, and what
+// it may read of them.
+template <int T>
+struct RowView {
+  static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
+  uint64_t index, first;
+  int k, step;  // first key of unit 0, keys between this thread's units
+  int pos, visible;
+  RowView() = default;
+  __device__ __forceinline__ RowView(const Rows<T>& r, const Team& t, int vpt)
+      : index(r.index), first(r.first + uint64_t((t.rank * uint32_t(vpt) * t.threads + t.tid) * 16u)),
+        k(int((t.rank * uint32_t(vpt) * t.threads + t.tid) * uint32_t(V)) - r.shift), step(int(t.threads) * V), pos(r.pos),
+        visible(r.visible) {}
+  __device__ __forceinline__ int key(int u) const { return k + u * step; }
+  __device__ __forceinline__ uint64_t offset(int u) const { return first + uint64_t(uint32_t(u * step * B)); }
+  __device__ __forceinline__ bool seen(int u) const { return key(u) < visible && key(u) + V > 0; }
+  __device__ __forceinline__ bool whole(int u) const { return key(u) >= 0 && key(u) + V <= visible; }
 
-// x[j] <- scale x[j] + bias where the key is visible, else -inf.
-template <int V>
-__device__ __forceinline__ void biased(const Row& r, const Window& win, const float* lut, float scale, int k0, float* x) {
-  const int rel = k0 - r.pos;
-  if (k0 >= r.visible || k0 + V <= 0) {
+  __device__ __forceinline__ void fetch(const BiasSoftmaxArgs& a, const void* p, uint64_t bytes, int u, uint32_t slot) const {
+    if (!seen(u)) return;
+    const char* from = static_cast<const char*>(p) + offset(u);
+    if (a.aligned && offset(u) + 16 <= bytes) {
+      copy_to_shared(slot, from);
+    } else {  // a tensor's last unit, or a tensor that starts inside 16 bytes: by elements
+      uint32_t w[4] = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = kNegInf;
-    return;
+      for (int j = 0; j < V; ++j) {
+        if (key(u) + j < 0 || key(u) + j >= visible) continue;
+        const uint32_t bits = B == 4 ? __ldg(reinterpret_cast<const uint32_t*>(from) + j)
+                                     : uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from) + j));
+        w[j * B / 4] |= bits << (8 * (j * B % 4));
+      }
+      st_shared(slot, make_uint4(w[0], w[1], w[2], w[3]));
+    }
   }
-  if (rel >= win.hi || rel + V - 1 <= -win.w) {
-    const float b = lut[rel >= win.hi ? win.size - 1 : 0];
+  // the unit's elements that belong to the row
+  __device__ __forceinline__ void store(const BiasSoftmaxArgs& a, int u, const uint64_t* v) const {
+    const int k0 = key(u), n = int(a.keys);
+    if (k0 >= n) return;
+    char* to = static_cast<char*>(a.out) + offset(u);
+    const uint4 o = act_narrow2<T>(v);
+    if (a.aligned && k0 >= 0 && k0 + V <= n) {
+      st_stream_v4(to, o);
+    } else {
+      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = __fmaf_rn(x[j], scale, b);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = __fmaf_rn(x[j], scale, lut[min(max(rel + j, -win.w), win.hi) + win.w]);
+      for (int j = 0; j < V; ++j) {
+        if (k0 + j < 0 || k0 + j >= n) continue;
+        if constexpr (B == 4) reinterpret_cast<uint32_t*>(to)[j] = w[j];
+        else reinterpret_cast<uint16_t*>(to)[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));
+      }
+    }
   }
-  if (k0 < 0 || k0 + V > r.visible) {
+  // v <- v where the key is visible, else `other`
+  __device__ __forceinline__ void mask(int u, float other, uint64_t* v) const {
+    if (whole(u)) return;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (k0 + j < 0 || k0 + j >= r.visible) x[j] = kNegInf;
+    for (int j = 0; j < V; j += 2) {
+      float lo, hi;
+      unpack2(v[j / 2], lo, hi);
+      const int at = key(u) + j;
+      v[j / 2] = pack2(at >= 0 && at < visible ? lo : other, at + 1 >= 0 && at + 1 < visible ? hi : other);
+    }
   }
-}
+  // x <- scale x + bias
+  __device__ __forceinline__ void logits(const Window<V>& win, uint32_t lut, float left, float right, uint64_t scale, int u,
+                                         uint64_t* x) const {
+    const int rel = key(u) - pos;
+    if (rel >= win.hi || rel + V - 1 <= -win.w) {
+      const uint64_t bias = both(rel >= win.hi ? right : left);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) x[j] = fma2(x[j], scale, bias);
+    } else {
+      const Places<V> at(lut, win.place(rel));
+#pragma unroll
+      for (int j = 0; j < V; j += 2)
+        x[j / 2] = fma2(x[j / 2], scale, pack2(ld_shared_f32(at(j)), ld_shared_f32(at(j + 1))));
+    }
+  }
+};
 
 // v <- exp(v - m); v may be -inf, m is not.
-template <int E>
-__device__ __forceinline__ void exp_minus(float (&v)[E], float m) {
-  if (fabsf(m) <= 0x1p100f) {
-    const float nm = -m * kLog2e;
+template <int N>
+__device__ __forceinline__ void exp_minus(uint64_t (&v)[N], float m) {
+  const bool direct = fabsf(m) <= 0x1p100f;
+  const uint64_t l = both(kLog2e), nm = both(direct ? -m * kLog2e : 0.0f);
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = ex2_approx(__fmaf_rn(v[i], kLog2e, nm));
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = ex2_approx((v[i] - m) * kLog2e);
+  for (int i = 0; i < N; ++i) {
+    uint64_t t;
+    if (direct) t = fma2(v[i], l, nm);
+    else t = mul2(add2(v[i], both(-m)), l);
+    float lo, hi;
+    unpack2(t, lo, hi);
+    v[i] = pack2(ex2_approx(lo), ex2_approx(hi));
   }
 }
 
-struct Task {
-  uint32_t head;
-  uint64_t pair, end, step;
-};
-__device__ __forceinline__ Task task_of(const BiasSoftmaxArgs& a, const Team& t) {
-  const bool warp_teams = a.shape.warp_teams;
-  const uint32_t place = blockIdx.x / t.ctas, chunk = place / a.heads;
-  const uint64_t n = a.batch * a.queries;
-  Task k;
-  k.head = place % a.heads;
-  k.pair = n * chunk / a.chunks + (warp_teams ? threadIdx.x >> 5 : 0);
-  k.end = n * (chunk + 1) / a.chunks;
-  k.step = warp_teams ? blockDim.x >> 5 : 1;
-  return k;
-}
+// 16-byte words of a thread for one row of one array.
+template <int T, int kElems>
+constexpr int row_words() { return kElems / act_vec<T>(); }
 
-template <int T, int VPT>
+template <int T, int E, bool kDrop>
 __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
-  constexpr int V = act_vec<T>(), E = V * VPT;
-  extern __shared__ float lut[];
+  constexpr int V = act_vec<T>(), U = E / V, P = E / 2, H = V / 2;
+  extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<2> sh;
   const Team t = team_of(a.shape.warp_teams);
-  const Window win = window_of(a);
-  Task task = task_of(a, t);
+  const Window<V> win(a);
+  Rows<T> rows(a, t);
+  const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
+  float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
+  const uint32_t lut_at = shared_address(lut);
+  const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
   pdl_enter();
   team_start(t);
-  fill_window(a, win, task.head, lut);
-  __syncthreads();
-  const DropRun run = drop_run(a.drop, a.seed);
-  const uint64_t total = a.batch * a.heads * a.queries * a.keys;
-  for (int parity = 0; task.pair < task.end; task.pair += task.step, parity ^= 1) {
-    const Row r = row_of<V>(a, task.head, task.pair);
-    auto key = [&](int q) { return int(((t.rank * VPT + q) * t.threads + t.tid) * uint32_t(V)) - r.shift; };
-    float e[E];
+  RowView<T> row;
+  auto fetch = [&](uint32_t slot) {
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) load_seen<T, V>(a, a.s, r, key(q), total, e + q * V);
+    for (int u = 0; u < U; ++u) row.fetch(a, a.s, bytes, u, slot + uint32_t(u) * pitch);
+  };
+  rows.start();
+  if (rows.left) {
+    row = RowView<T>(rows, t, U);
+    fetch(ring);
+  }
+  copy_async_commit();
+  DropRun run{};
+  if constexpr (kDrop) run = drop_run(a.drop, a.seed);
+  fill_window(a, win, rows.head, lut);
+  __syncthreads();
+  const float left = lut[0], right = lut[win.word(win.places() - 1)];
+  const uint64_t scale = both(a.scale);
+  // the teams of a warp go on together: one without a row works on its last
+  // again, without writing
+  bool on = rows.left > 0;
+  const bool two = a.ring_rows == 2;  // a row ahead; else the next one is fetched when this one is read
+  for (uint32_t turn = 0; __any_sync(0xffffffffu, on); ++turn) {
+    const uint32_t slot = ring + (two ? turn & 1u : 0u) * (uint32_t(U) * pitch);
+    const int parity = int(turn & 1u);
+    const RowView<T> r = row;
+    const bool here = on;
+    if (on) {
+      rows.next();
+      on = rows.left > 0;
+      if (on) {
+        row = RowView<T>(rows, t, U);
+        if (two) fetch(ring + ((turn & 1u) ^ 1u) * (uint32_t(U) * pitch));
+      }
+    }
+    copy_async_commit();
+    if (two) copy_async_wait<1>();
+    else copy_async_wait<0>();
+    uint64_t e[P];
     float m = kNegInf;
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      biased<V>(r, win, lut, a.scale, key(q), e + q * V);
+    for (int u = 0; u < U; ++u) {
+      uint64_t* x = e + u * H;
+      if (here && r.seen(u)) {
+        act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), x);
+        r.logits(win, lut_at, left, right, scale, u, x);
+        r.mask(u, kNegInf, x);
 #pragma unroll
-      for (int j = 0; j < V; ++j) m = fmaxf(m, e[q * V + j]);
+        for (int j = 0; j < H; ++j) {
+          float lo, hi;
+          unpack2(x[j], lo, hi);
+          m = fmaxf(m, fmaxf(lo, hi));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < H; ++j) x[j] = both(kNegInf);
+      }
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int d = 16; d; d >>= 1)
+      if (uint32_t(d) < t.lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float base = m == kNegInf ? 0.0f : m;  // nothing visible: every 2^x below is 0
-    float s = 0.0f;
-    exp_minus<E>(e, base);
+    exp_minus(e, base);
+    uint64_t s2 = e[0], s3 = e[1];
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += e[i];
+    for (int i = 2; i < P; i += 2) {
+      s2 = add2(s2, e[i]);
+      s3 = add2(s3, e[i + 1]);
+    }
+    float s = sum2(add2(s2, s3));
 #pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    for (int d = 16; d; d >>= 1)
+      if (uint32_t(d) < t.lanes) s += __shfl_xor_sync(0xffffffffu, s, d);
     // the team's maximum and sum from the warps' own
     float top = base, sum = s, factor = 1.0f;
     const uint32_t records = t.warps * t.ctas;
@@ -230,96 +363,179 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
       for (uint32_t k = 0; k < records; ++k) top = fmaxf(top, sh.v[parity][k][0]);
       if (top == kNegInf) top = 0.0f;
       sum = 0.0f;
-      for (uint32_t k = 0; k < records; ++k) sum = __fmaf_rn(sh.v[parity][k][1], ex2_approx((sh.v[parity][k][0] - top) * kLog2e), sum);
+      for (uint32_t k = 0; k < records; ++k)
+        sum = __fmaf_rn(sh.v[parity][k][1], ex2_approx((sh.v[parity][k][0] - top) * kLog2e), sum);
       factor = ex2_approx((m - top) * kLog2e);
     }
     factor = sum == 0.0f ? 0.0f : factor * __frcp_rn(sum);
+    if (!two && on) fetch(ring);
+    if (!here) continue;
     if (t.tid == 0 && t.rank == 0) a.lse[r.index] = sum == 0.0f ? kNegInf : top + logf(sum);
+    const uint64_t by = both(kDrop ? factor * run.scale : factor);
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      const int k0 = key(q);
-      float* v = e + q * V;
-      const bool seen = k0 < r.visible && k0 + V > 0;
+    for (int u = 0; u < U; ++u) {
+      uint64_t* x = e + u * H;
+      if (r.seen(u)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = k0 + j >= 0 && k0 + j < r.visible ? v[j] * factor : 0.0f;
-      if (a.drop.on && seen) drop_unit<V>(run, r.first + uint64_t(int64_t(k0) + r.shift), v);
-      store_row<T, V>(a, r, k0, v);
+        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], by);
+        if constexpr (kDrop) {
+          const uint64_t i[1] = {r.offset(u) / dtype_bytes(T)};
+          bool keep[V];
+          drop_keep<1, V>(run, i, keep);
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            float lo, hi;
+            unpack2(x[j], lo, hi);
+            x[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
+          }
+        }
+        r.mask(u, 0.0f, x);  // a row with a NaN has a NaN factor
+      } else {
+#pragma unroll
+        for (int j = 0; j < H; ++j) x[j] = 0;
+      }
+      r.store(a, u, x);
     }
   }
 }
 
-template <int T, int VPT>
+template <int T, int E, bool kDrop>
 __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
-  constexpr int V = act_vec<T>(), E = V * VPT;
-  extern __shared__ float lut[];
+  constexpr int V = act_vec<T>(), U = E / V, P = E / 2, H = V / 2;
+  extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<1> sh;
   __shared__ float ends[2][kTeamThreads / 32];
-  const bool warp_teams = a.shape.warp_teams;
   const Team t = team_of(a.shape.warp_teams);
-  const Window win = window_of(a);
-  Task task = task_of(a, t);
-  const int teams = warp_teams ? int(blockDim.x >> 5) : 1;
-  float* const sums = lut + win.size;  // the teams' windows
-  float* const mine = sums + (warp_teams ? int(threadIdx.x >> 5) : 0) * win.size;
+  const Window<V> win(a);
+  Rows<T> rows(a, t);
+  const int teams = a.shape.warp_teams ? int(blockDim.x / t.threads) : 1;
+  const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
+  float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * 2 * row_words<T, E>() * blockDim.x);
+  float* const sums = lut + win.words();  // the teams' windows
+  const uint32_t lut_at = shared_address(lut),
+                 mine = shared_address(sums + (a.shape.warp_teams ? int(threadIdx.x / t.threads) : 0) * win.words());
+  const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
   pdl_enter();
   team_start(t);
-  fill_window(a, win, task.head, lut);
-  for (int i = int(threadIdx.x); i < teams * win.size; i += int(blockDim.x)) sums[i] = 0.0f;
-  __syncthreads();
-  const DropRun run = drop_run(a.drop, a.seed);
-  const uint64_t total = a.batch * a.heads * a.queries * a.keys;
-  float left = 0.0f, right = 0.0f;  // dl at rel <= -W and at rel >= hi
-  for (int parity = 0; task.pair < task.end; task.pair += task.step, parity ^= 1) {
-    const Row r = row_of<V>(a, task.head, task.pair);
-    auto key = [&](int q) { return int(((t.rank * VPT + q) * t.threads + t.tid) * uint32_t(V)) - r.shift; };
-    float p[E], d[E];
+  RowView<T> row;
+  float row_lse = 0.0f;
+  auto fetch = [&](uint32_t slot) {
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      load_seen<T, V>(a, a.s, r, key(q), total, p + q * V);
-      load_seen<T, V>(a, a.dp, r, key(q), total, d + q * V);
+    for (int u = 0; u < U; ++u) {
+      row.fetch(a, a.s, bytes, u, slot + uint32_t(2 * u) * pitch);
+      row.fetch(a, a.dp, bytes, u, slot + uint32_t(2 * u + 1) * pitch);
     }
-    const float lse = __ldg(a.lse_in + r.index);
-    const float base = lse == kNegInf ? 0.0f : lse;  // all logits are -inf then, and every P is 0
-    float dot[1] = {0.0f};
-#pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      const int k0 = key(q);
-      biased<V>(r, win, lut, a.scale, k0, p + q * V);
-      if (a.drop.on && k0 < r.visible && k0 + V > 0)
-        drop_unit<V>(run, r.first + uint64_t(int64_t(k0) + r.shift), d + q * V);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int i = q * V + j;
-        const bool seen = k0 + j >= 0 && k0 + j < r.visible;
-        d[i] = seen ? d[i] : 0.0f;
+    row_lse = __ldg(a.lse_in + row.index);
+  };
+  rows.start();
+  if (rows.left) {
+    row = RowView<T>(rows, t, U);
+    fetch(ring);
+  }
+  copy_async_commit();
+  DropRun run{};
+  if constexpr (kDrop) run = drop_run(a.drop, a.seed);
+  fill_window(a, win, rows.head, lut);
+  for (int i = int(threadIdx.x); i < teams * win.words(); i += int(blockDim.x)) sums[i] = 0.0f;
+  __syncthreads();
+  const float bias_left = lut[0], bias_right = lut[win.word(win.places() - 1)];
+  const uint64_t scale = both(a.scale);
+  const float drop_scale = kDrop ? run.scale : 1.0f;
+  float left = 0.0f, right = 0.0f;  // dl of units wholly at rel <= -W, or at rel >= hi
+  bool on = rows.left > 0;
+  const bool two = a.ring_rows == 2;
+  for (uint32_t turn = 0; __any_sync(0xffffffffu, on); ++turn) {
+    const uint32_t slot = ring + (two ? turn & 1u : 0u) * (uint32_t(2 * U) * pitch);
+    const RowView<T> r = row;
+    const bool here = on;
+    const float lse = row_lse, base = lse == kNegInf ? 0.0f : lse;  // all logits are -inf then, and every P is 0
+    if (on) {
+      rows.next();
+      on = rows.left > 0;
+      if (on) {
+        row = RowView<T>(rows, t, U);
+        if (two) fetch(ring + ((turn & 1u) ^ 1u) * (uint32_t(2 * U) * pitch));
       }
     }
-    exp_minus<E>(p, base);
+    copy_async_commit();
+    if (two) copy_async_wait<1>();
+    else copy_async_wait<0>();
+    uint64_t p[P], d[P];
 #pragma unroll
-    for (int i = 0; i < E; ++i) dot[0] = __fmaf_rn(p[i], d[i], dot[0]);
-    team_sum<1>(t, sh, parity, dot);
-    if (warp_teams) __syncwarp();  // the lanes' adds of the row before are done
-    float row_left = 0.0f, row_right = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      uint64_t *x = p + u * H, *y = d + u * H;
+      if (here && r.seen(u)) {
+        act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), x);
+        act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), y);
+        r.logits(win, lut_at, bias_left, bias_right, scale, u, x);
+        r.mask(u, kNegInf, x);
+        r.mask(u, 0.0f, y);
+        if constexpr (kDrop) {
+          const uint64_t i[1] = {r.offset(u) / dtype_bytes(T)};
+          bool keep[V];
+          drop_keep<1, V>(run, i, keep);
 #pragma unroll
-    for (int q = 0; q < VPT; ++q) {
-      const int k0 = key(q), rel = k0 - r.pos;
-      float o[V];
+          for (int j = 0; j < H; ++j) {
+            float lo, hi;
+            unpack2(y[j], lo, hi);
+            y[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
+          }
+        }
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int i = q * V + j;
-        const bool seen = k0 + j >= 0 && k0 + j < r.visible;
-        p[i] = seen ? p[i] * (d[i] - dot[0]) : 0.0f;
-        o[j] = p[i] * a.scale;
-        if (seen) {
-          if (rel + j <= -win.w) row_left += p[i];
-          else if (rel + j >= win.hi) row_right += p[i];
-          else mine[rel + j + win.w] += p[i];
+        for (int j = 0; j < H; ++j) {
+          x[j] = both(kNegInf);
+          y[j] = 0;
         }
       }
-      store_row<T, V>(a, r, k0, o);
     }
-    left += row_left;
-    right += row_right;
+    exp_minus(p, base);
+    uint64_t s2 = mul2(p[0], d[0]), s3 = mul2(p[1], d[1]);
+#pragma unroll
+    for (int i = 2; i < P; i += 2) {
+      s2 = fma2(p[i], d[i], s2);
+      s3 = fma2(p[i + 1], d[i + 1], s3);
+    }
+    float dot[1] = {sum2(add2(s2, s3))};
+    team_sum<1>(t, sh, int(turn & 1u), dot);
+    if (a.shape.warp_teams) __syncwarp();  // the lanes' adds of the row before are done
+    if (!two && on) fetch(ring);
+    if (!here) continue;
+    // dl = P (D(dp) - sum): the dropout's scale enters here
+    const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint64_t *x = p + u * H, o[H];
+      if (r.seen(u)) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u * H + j], by, minus));
+        r.mask(u, 0.0f, x);  // a NaN sum stays with the keys that are seen
+        const int rel = r.key(u) - r.pos;
+        if (rel >= win.hi || rel + V - 1 <= -win.w) {
+          uint64_t v = x[0];
+#pragma unroll
+          for (int j = 1; j < H; ++j) v = add2(v, x[j]);
+          const float f = sum2(v);
+          left += rel >= win.hi ? 0.0f : f;
+          right += rel >= win.hi ? f : 0.0f;
+        } else {
+          const Places<V> at(mine, win.place(rel));
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            float lo, hi;
+            unpack2(x[j], lo, hi);
+            st_shared_f32(at(2 * j), ld_shared_f32(at(2 * j)) + lo);
+            st_shared_f32(at(2 * j + 1), ld_shared_f32(at(2 * j + 1)) + hi);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < H; ++j) o[j] = mul2(x[j], scale);
+      } else {
+#pragma unroll
+        for (int j = 0; j < H; ++j) o[j] = 0;
+      }
+      r.store(a, u, o);
+    }
   }
   // fold the windows by bucket
 #pragma unroll
@@ -337,15 +553,17 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   for (int b = warp; b < int(a.buckets); b += warps) {
     const bool ahead = b >= side;  // rel > 0
     const int j = ahead ? b - side : b;
-    // distances [n0, n1) of the bucket, inside the window
-    const int n0 = max(j ? a.thresholds[j - 1] : 0, ahead ? 1 : 0), n1 = j < a.n_thresholds ? a.thresholds[j] : win.w;
-    float v = 0.0f;
-    for (int k = 0; k < teams; ++k)
-      for (int n = n0 + lane; n < n1; n += 32) {
-        const int at = ahead ? win.w + n : win.w - n;
-        if (at > 0 && at < win.size - 1) v += sums[k * win.size + at];
-      }
     const bool is_left = !ahead && j == a.n_thresholds, is_right = a.bidirectional ? ahead && j == a.n_thresholds : j == 0;
+    // the bucket's distances [n0, n1): from the last threshold on the V - 1 places
+    // beyond the window too, as have the keys ahead where only distances behind count
+    const int n0 = max(j ? a.thresholds[j - 1] : 0, ahead ? 1 : 0);
+    const int n1 = j < a.n_thresholds ? a.thresholds[j] : win.w + V;
+    float v = 0.0f;
+    for (int k = 0; k < teams; ++k) {
+      const float* at = sums + k * win.words();
+      for (int n = n0 + lane; n < n1; n += 32) v += at[win.word(win.place(ahead ? n : -n))];
+      if (!a.bidirectional && j == 0 && lane > 0 && lane < V) v += at[win.word(win.place(lane))];
+    }
     if (lane < warps) v += (is_left ? ends[0][lane] : 0.0f) + (is_right ? ends[1][lane] : 0.0f);
 #pragma unroll
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -372,29 +590,33 @@ __global__ void __launch_bounds__(256) bias_table_join_kernel(const float* __res
   if (lane == 0) dtable[out] = float(v);
 }
 
-template <int T>
+template <int T, bool kDrop>
 const void* kernel_of_type(int elems, bool grad) {
-  constexpr int V = act_vec<T>();
   if (grad)
-    return elems == 8    ? (const void*)bias_softmax_grad_kernel<T, 8 / V>
-           : elems == 16 ? (const void*)bias_softmax_grad_kernel<T, 16 / V>
-                         : (const void*)bias_softmax_grad_kernel<T, 32 / V>;
-  return elems == 8    ? (const void*)bias_softmax_kernel<T, 8 / V>
-         : elems == 16 ? (const void*)bias_softmax_kernel<T, 16 / V>
-                       : (const void*)bias_softmax_kernel<T, 32 / V>;
+    return elems == 8    ? (const void*)bias_softmax_grad_kernel<T, 8, kDrop>
+           : elems == 16 ? (const void*)bias_softmax_grad_kernel<T, 16, kDrop>
+                         : (const void*)bias_softmax_grad_kernel<T, 32, kDrop>;
+  return elems == 8    ? (const void*)bias_softmax_kernel<T, 8, kDrop>
+         : elems == 16 ? (const void*)bias_softmax_kernel<T, 16, kDrop>
+                       : (const void*)bias_softmax_kernel<T, 32, kDrop>;
+}
+template <bool kDrop>
+const void* kernel_of(const BiasSoftmaxArgs& a, bool grad) {
+  return a.type == kF32   ? kernel_of_type<kF32, kDrop>(a.shape.elems, grad)
+         : a.type == kF16 ? kernel_of_type<kF16, kDrop>(a.shape.elems, grad)
+                          : kernel_of_type<kBF16, kDrop>(a.shape.elems, grad);
 }
 const void* kernel_for(const BiasSoftmaxArgs& a, bool grad) {
-  return a.type == kF32 ? kernel_of_type<kF32>(a.shape.elems, grad)
-         : a.type == kF16 ? kernel_of_type<kF16>(a.shape.elems, grad) : kernel_of_type<kBF16>(a.shape.elems, grad);
+  return a.drop.on ? kernel_of<true>(a, grad) : kernel_of<false>(a, grad);
 }
 
-// Windows above the default 48 KB (static arrays included) need the kernel's limit raised.
+// Shared memory above the default 48 KB (static arrays included) needs the kernel's limit raised.
 cudaError_t allow_shared(const void* kernel, uint32_t bytes) {
   return bytes <= 32 * 1024 ? cudaSuccess
                             : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
 
-constexpr uint32_t kWindowBytes = 192 * 1024;  // dynamic shared memory of a CTA at most
+constexpr uint32_t kSharedBytes = 216 * 1024;  // dynamic shared memory of a CTA at most
 
 }  // namespace
 
@@ -405,8 +627,9 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   const uint64_t span = keys % v ? keys + v - 1 : keys;
   TeamShape s{0, kWarpTeamThreads, 1, 32};
   if (rows >= uint64_t(sms) * 8 && span <= 32 * 32) {
-    s.warp_teams = 32;
-    s.elems = span <= 32 * 8 ? 8 : span <= 32 * 16 ? 16 : 32;
+    s.elems = span <= 32 * 16 ? 16 : 32;
+    s.warp_teams = 4;
+    while (span > uint64_t(s.warp_teams) * uint64_t(s.elems)) s.warp_teams *= 2;
     return s;
   }
   if (rows < uint64_t(sms) * 2) s.elems = 8;  // few rows: more threads for each
@@ -422,13 +645,21 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
 }
 
 void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad) {
-  const uint32_t window = uint32_t(window_of(*a).size) * 4;
-  uint32_t teams = a->shape.warp_teams ? uint32_t(a->shape.threads) / 32 : 1;
-  if (grad && a->shape.warp_teams) {
-    while (teams > 1 && window * (1 + teams) > kWindowBytes) --teams;
-    a->shape.threads = int(teams) * 32;
+  const uint32_t window = uint32_t(a->type == kF32 ? Window<4>(*a).words() : Window<8>(*a).words()) * 4;
+  const uint32_t row = (grad ? 2u : 1u) * uint32_t(a->shape.elems) * (a->type == kF32 ? 4u : 2u);  // bytes of a thread
+  a->ring_rows = 2;
+  auto total = [&] {
+    return a->ring_rows * row * uint32_t(a->shape.threads) +
+           (1 + (grad ? uint32_t(team_count(a->shape)) : 0u)) * window;
+  };
+  // wide windows leave room for fewer teams, the longest f32 rows for one row at a time
+  while (a->shape.warp_teams && total() > kSharedBytes / 2) {
+    if (a->shape.threads > 32) a->shape.threads -= 32;
+    else if (a->shape.warp_teams < 32) a->shape.warp_teams *= 2;
+    else break;
   }
-  a->shared_bytes = window * (grad ? 1 + teams : 1);
+  if (total() > kSharedBytes) a->ring_rows = 1;
+  a->shared_bytes = total();
 }
 
 cudaError_t bias_softmax_occupancy(const BiasSoftmaxArgs& a, bool grad, int* blocks_per_sm) {

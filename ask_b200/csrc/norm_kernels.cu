@@ -36,13 +36,6 @@ namespace {
 constexpr int kWarpTeamThreads = 256;
 constexpr int kElems = 16;  // row elements a thread holds
 
-__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
-__device__ __forceinline__ float sum2(uint64_t v) {
-  float lo, hi;
-  unpack2(v, lo, hi);
-  return lo + hi;
-}
-
 // A row array in flight: every thread copies the 16-byte words of its own
 // units into its own places of a ring in shared memory (cp.async) and reads
 // them back, so no barrier is needed, rows are fetched kStages - 1 ahead, and no
@@ -53,22 +46,6 @@ struct Ring {
   static constexpr int V = act_vec<T>(), Q = kElems / V, W = kAnywhere ? 2 : 1;
   static constexpr int kWords = Q * W;  // 16-byte words of one thread, array and stage
 };
-
-// Shared memory by its 32-bit address.
-__device__ __forceinline__ uint32_t shared_address(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
-  return r;
-}
-__device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ void copy_to_shared(uint32_t at, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-}
 
 // The team's columns of a row, as the thread holds them: units of 16 bytes, as
 // f32 pairs.  A row is named by the byte offset of this thread's first column.

@@ -1048,6 +1048,7 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
   const uint64_t heads = checked_count(r.at("heads"), "heads"), keys = checked_count(r.at("keys"), "keys");
   a.queries = checked_count(r.at("queries"), "queries");
   if (heads > (1u << 20)) fail(ASK_B200_E_UNSUPPORTED, "at most 2^20 heads");
+  if (a.batch > (uint64_t(1) << 30)) fail(ASK_B200_E_UNSUPPORTED, "at most 2^30 sequences");
   if (a.queries > (uint64_t(1) << 30)) fail(ASK_B200_E_UNSUPPORTED, "at most 2^30 queries");
   if (keys > kBiasMaxKeys) fail(ASK_B200_E_UNSUPPORTED, "at most " + std::to_string(kBiasMaxKeys) + " keys");
   a.heads = uint32_t(heads);
