@@ -107,93 +107,96 @@ __device__ __forceinline__ void fill_window(const BiasSoftmaxArgs& a, const Wind
 }
 
 // The rows of a team, one after the other: pairs (batch, query) of one head.
-template <int T>
+// kEven: rows are whole 16-byte units (keys a multiple of V, aligned tensors).
+template <int T, bool kEven>
 struct Rows {
-  static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
-  const BiasSoftmaxArgs& a;
+  static constexpr int V = act_vec<T>();
   uint32_t head, step, b, q;
-  uint64_t left;          // rows from this one on, in steps
-  int length, place;      // of the sequence: keys in use, position of its query 0
-  // of the row
-  uint64_t index, first;  // byte offset of its first unit
-  int shift;              // elements of that unit before the row
-  int pos, visible;       // query position; keys [0, visible) are seen
+  uint32_t left;       // rows from this one on
+  int length, place;   // of the sequence: keys in use, position of its query 0
+  uint64_t index;      // of the row
+  uint32_t mine;       // this thread's first unit, in elements of a row
 
-  __device__ __forceinline__ Rows(const BiasSoftmaxArgs& args, const Team& t) : a(args) {
+  __device__ __forceinline__ Rows(const BiasSoftmaxArgs& a, const Team& t, int units) {
     const uint32_t cta = blockIdx.x / t.ctas, chunk = cta / a.heads;
     const uint64_t n = a.batch * a.queries, begin = n * chunk / a.chunks, end = n * (chunk + 1) / a.chunks;
     const uint32_t team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
     head = cta % a.heads;
     step = a.shape.warp_teams ? blockDim.x / t.threads : 1;
-    left = begin + team < end ? (end - begin - team + step - 1) / step : 0;
+    left = begin + team < end ? uint32_t((end - begin - team + step - 1) / step) : 0;
     b = uint32_t((begin + team) / a.queries);
     q = uint32_t((begin + team) % a.queries);
+    mine = (t.rank * uint32_t(units) * t.threads + t.tid) * uint32_t(V);
+    if (left) sequence(a);
   }
-  __device__ __forceinline__ void sequence() {
+  __device__ __forceinline__ void sequence(const BiasSoftmaxArgs& a) {
     length = int(a.keys);
     place = 0;
     if (a.lengths) length = max(min(__ldg(a.lengths + b), length), 0);
     if (a.offsets) place = __ldg(a.offsets + b);
-  }
-  __device__ __forceinline__ void locate() {
     index = (uint64_t(b) * a.heads + head) * a.queries + q;
-    const uint64_t e = index * a.keys;
-    shift = int(uint32_t(e) & uint32_t(V - 1));
-    first = (e - uint64_t(shift)) * B;
-    const int64_t at = int64_t(place) + int64_t(q);
-    visible = length;
-    if (a.causal) visible = int(max(min(int64_t(length), at + 1), int64_t(0)));
-    // far positions meet only the window's ends, whatever their distance
-    pos = int(max(min(at, int64_t(1) << 30), -(int64_t(1) << 30)));
   }
-  // to be called once before the first row, then to go on
-  __device__ __forceinline__ void start() {
-    if (left) {
-      sequence();
-      locate();
-    }
-  }
-  __device__ __forceinline__ void next() {
+  __device__ __forceinline__ void next(const BiasSoftmaxArgs& a) {
     if (--left == 0) return;
     q += step;
-    if (q >= a.queries) {
+    index += step;
+    if (q >= uint32_t(a.queries)) {
       const uint32_t n = q / uint32_t(a.queries);
       b += n;
       q -= n * uint32_t(a.queries);
-      sequence();
+      sequence(a);
     }
-    locate();
   }
 };
 
-// One row of a team in flight or at work: which units the thread has, and what
-// it may read of them.
-template <int T>
+// One row, in flight or at work, as a thread sees it: unit u begins at key
+// k + u * (keys between units) and at byte offset off + u * (bytes between units).
 struct RowView {
+  uint64_t off;
+  int k, visible, pos;  // keys [0, visible) are seen; position of the query
+};
+template <int T, bool kEven>
+struct Units {
   static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
-  uint64_t index, first;
-  int k, step;  // first key of unit 0, keys between this thread's units
-  int pos, visible;
-  RowView() = default;
-  __device__ __forceinline__ RowView(const Rows<T>& r, const Team& t, int vpt)
-      : index(r.index), first(r.first + uint64_t((t.rank * uint32_t(vpt) * t.threads + t.tid) * 16u)),
-        k(int((t.rank * uint32_t(vpt) * t.threads + t.tid) * uint32_t(V)) - r.shift), step(int(t.threads) * V), pos(r.pos),
-        visible(r.visible) {}
-  __device__ __forceinline__ int key(int u) const { return k + u * step; }
-  __device__ __forceinline__ uint64_t offset(int u) const { return first + uint64_t(uint32_t(u * step * B)); }
-  __device__ __forceinline__ bool seen(int u) const { return key(u) < visible && key(u) + V > 0; }
-  __device__ __forceinline__ bool whole(int u) const { return key(u) >= 0 && key(u) + V <= visible; }
+  int keys;
+  int key_step;        // keys between a thread's units
+  __device__ __forceinline__ Units(const BiasSoftmaxArgs& a, const Team& t) : keys(int(a.keys)), key_step(int(t.threads) * V) {}
 
-  __device__ __forceinline__ void fetch(const BiasSoftmaxArgs& a, const void* p, uint64_t bytes, int u, uint32_t slot) const {
-    if (!seen(u)) return;
-    const char* from = static_cast<const char*>(p) + offset(u);
-    if (a.aligned && offset(u) + 16 <= bytes) {
+  __device__ __forceinline__ RowView view(const BiasSoftmaxArgs& a, const Rows<T, kEven>& rows) const {
+    RowView r;
+    uint64_t e = rows.index * a.keys + rows.mine;
+    r.k = int(rows.mine);
+    if constexpr (!kEven) {  // the tensor's own units: the first begins before the row
+      const uint32_t shift = uint32_t(e) & uint32_t(V - 1);
+      e -= shift;
+      r.k -= int(shift);
+    }
+    r.off = e * B;
+    const int64_t at = int64_t(rows.place) + int64_t(rows.q);
+    r.visible = rows.length;
+    if (a.causal) r.visible = int(max(min(int64_t(rows.length), at + 1), int64_t(0)));
+    // far positions meet only the window's ends, whatever their distance
+    r.pos = int(max(min(at, int64_t(1) << 30), -(int64_t(1) << 30)));
+    return r;
+  }
+  __device__ __forceinline__ int key(const RowView& r, int u) const { return r.k + u * key_step; }
+  __device__ __forceinline__ uint64_t offset(const RowView& r, int u) const { return r.off + uint32_t(u * key_step * B); }
+  __device__ __forceinline__ bool seen(const RowView& r, int u) const {
+    return key(r, u) < r.visible && (kEven || key(r, u) > -V);
+  }
+
+  __device__ __forceinline__ void fetch(const BiasSoftmaxArgs& a, const void* p, uint64_t bytes, const RowView& r, int u,
+                                        uint32_t slot) const {
+    if (!seen(r, u)) return;
+    const char* from = static_cast<const char*>(p) + offset(r, u);
+    if (kEven || (a.aligned && offset(r, u) + 16 <= bytes)) {
       copy_to_shared(slot, from);
     } else {  // a tensor's last unit, or a tensor that starts inside 16 bytes: by elements
       uint32_t w[4] = {};
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (key(u) + j < 0 || key(u) + j >= visible) continue;
+        const int at = key(r, u) + j;
+        if (at < 0 || at >= r.visible) continue;
         const uint32_t bits = B == 4 ? __ldg(reinterpret_cast<const uint32_t*>(from) + j)
                                      : uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from) + j));
         w[j * B / 4] |= bits << (8 * (j * B % 4));
@@ -202,38 +205,39 @@ struct RowView {
     }
   }
   // the unit's elements that belong to the row
-  __device__ __forceinline__ void store(const BiasSoftmaxArgs& a, int u, const uint64_t* v) const {
-    const int k0 = key(u), n = int(a.keys);
-    if (k0 >= n) return;
-    char* to = static_cast<char*>(a.out) + offset(u);
-    const uint4 o = act_narrow2<T>(v);
-    if (a.aligned && k0 >= 0 && k0 + V <= n) {
+  __device__ __forceinline__ void store(const BiasSoftmaxArgs& a, const RowView& r, int u, const uint4& o) const {
+    const int k0 = key(r, u);
+    if (k0 >= keys) return;
+    char* to = static_cast<char*>(a.out) + offset(r, u);
+    if (kEven || (a.aligned && k0 >= 0 && k0 + V <= keys)) {
       st_stream_v4(to, o);
     } else {
       const uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (k0 + j < 0 || k0 + j >= n) continue;
+        if (k0 + j < 0 || k0 + j >= keys) continue;
         if constexpr (B == 4) reinterpret_cast<uint32_t*>(to)[j] = w[j];
         else reinterpret_cast<uint16_t*>(to)[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));
       }
     }
   }
   // v <- v where the key is visible, else `other`
-  __device__ __forceinline__ void mask(int u, float other, uint64_t* v) const {
-    if (whole(u)) return;
+  __device__ __forceinline__ void mask(const RowView& r, int u, float other, uint64_t* v) const {
+    const int k0 = key(r, u);
+    if ((kEven || k0 >= 0) && k0 + V <= r.visible) return;
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       float lo, hi;
       unpack2(v[j / 2], lo, hi);
-      const int at = key(u) + j;
-      v[j / 2] = pack2(at >= 0 && at < visible ? lo : other, at + 1 >= 0 && at + 1 < visible ? hi : other);
+      const int at = k0 + j;
+      v[j / 2] = pack2((kEven || at >= 0) && at < r.visible ? lo : other,
+                       (kEven || at + 1 >= 0) && at + 1 < r.visible ? hi : other);
     }
   }
   // x <- scale x + bias
-  __device__ __forceinline__ void logits(const Window<V>& win, uint32_t lut, float left, float right, uint64_t scale, int u,
-                                         uint64_t* x) const {
-    const int rel = key(u) - pos;
+  __device__ __forceinline__ void logits(const RowView& r, const Window<V>& win, uint32_t lut, float left, float right,
+                                         uint64_t scale, int u, uint64_t* x) const {
+    const int rel = key(r, u) - r.pos;
     if (rel >= win.hi || rel + V - 1 <= -win.w) {
       const uint64_t bias = both(rel >= win.hi ? right : left);
 #pragma unroll
@@ -247,18 +251,34 @@ struct RowView {
   }
 };
 
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float lg2_approx(float v) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // v <- exp(v - m); v may be -inf, m is not.
 template <int N>
-__device__ __forceinline__ void exp_minus(uint64_t (&v)[N], float m) {
-  const bool direct = fabsf(m) <= 0x1p100f;
-  const uint64_t l = both(kLog2e), nm = both(direct ? -m * kLog2e : 0.0f);
+__device__ __forceinline__ void exp_minus(uint64_t* v, float m) {
+  const uint64_t l = both(kLog2e);
+  if (fabsf(m) <= 0x1p100f) {
+    const uint64_t nm = both(-m * kLog2e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fma2(v[i], l, nm);
+  } else {
+    const uint64_t nm = both(-m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = mul2(add2(v[i], nm), l);
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    uint64_t t;
-    if (direct) t = fma2(v[i], l, nm);
-    else t = mul2(add2(v[i], both(-m)), l);
     float lo, hi;
-    unpack2(t, lo, hi);
+    unpack2(v[i], lo, hi);
     v[i] = pack2(ex2_approx(lo), ex2_approx(hi));
   }
 }
@@ -267,28 +287,31 @@ __device__ __forceinline__ void exp_minus(uint64_t (&v)[N], float m) {
 template <int T, int kElems>
 constexpr int row_words() { return kElems / act_vec<T>(); }
 
-template <int T, int E, bool kDrop>
+template <int T, int E, bool kDrop, bool kEven>
 __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
-  constexpr int V = act_vec<T>(), U = E / V, P = E / 2, H = V / 2;
+  constexpr int V = act_vec<T>(), U = E / V, H = V / 2;
   extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<2> sh;
   const Team t = team_of(a.shape.warp_teams);
   const Window<V> win(a);
-  Rows<T> rows(a, t);
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
   const uint32_t lut_at = shared_address(lut);
   const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
+  const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
-  RowView<T> row;
+  Rows<T, kEven> rows(a, t, U);
+  RowView row{};
+  uint64_t index = 0;
   auto fetch = [&](uint32_t slot) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) row.fetch(a, a.s, bytes, u, slot + uint32_t(u) * pitch);
+    for (int u = 0; u < U; ++u) units.fetch(a, a.s, bytes, row, u, slot + uint32_t(u) * pitch);
   };
-  rows.start();
-  if (rows.left) {
-    row = RowView<T>(rows, t, U);
+  bool on = rows.left > 0;
+  if (on) {
+    row = units.view(a, rows);
+    index = rows.index;
     fetch(ring);
   }
   copy_async_commit();
@@ -298,56 +321,55 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   __syncthreads();
   const float left = lut[0], right = lut[win.word(win.places() - 1)];
   const uint64_t scale = both(a.scale);
-  // the teams of a warp go on together: one without a row works on its last
-  // again, without writing
-  bool on = rows.left > 0;
   const bool two = a.ring_rows == 2;  // a row ahead; else the next one is fetched when this one is read
+  // the teams of a warp go on together while one of them has a row
   for (uint32_t turn = 0; __any_sync(0xffffffffu, on); ++turn) {
     const uint32_t slot = ring + (two ? turn & 1u : 0u) * (uint32_t(U) * pitch);
     const int parity = int(turn & 1u);
-    const RowView<T> r = row;
+    const RowView r = row;
+    const uint64_t this_index = index;
     const bool here = on;
     if (on) {
-      rows.next();
+      rows.next(a);
       on = rows.left > 0;
       if (on) {
-        row = RowView<T>(rows, t, U);
+        row = units.view(a, rows);
+        index = rows.index;
         if (two) fetch(ring + ((turn & 1u) ^ 1u) * (uint32_t(U) * pitch));
       }
     }
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
-    uint64_t e[P];
+    uint64_t e[U][H];
     float m = kNegInf;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint64_t* x = e + u * H;
-      if (here && r.seen(u)) {
-        act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), x);
-        r.logits(win, lut_at, left, right, scale, u, x);
-        r.mask(u, kNegInf, x);
+      if (!here || !units.seen(r, u)) continue;
+      act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), e[u]);
+      units.logits(r, win, lut_at, left, right, scale, u, e[u]);
+      units.mask(r, u, kNegInf, e[u]);
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-          float lo, hi;
-          unpack2(x[j], lo, hi);
-          m = fmaxf(m, fmaxf(lo, hi));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < H; ++j) x[j] = both(kNegInf);
+      for (int j = 0; j < H; ++j) {
+        float lo, hi;
+        unpack2(e[u][j], lo, hi);
+        m = fmaxf(m, fmaxf(lo, hi));
       }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
       if (uint32_t(d) < t.lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float base = m == kNegInf ? 0.0f : m;  // nothing visible: every 2^x below is 0
-    exp_minus(e, base);
-    uint64_t s2 = e[0], s3 = e[1];
+    uint64_t s2 = 0, s3 = 0;
 #pragma unroll
-    for (int i = 2; i < P; i += 2) {
-      s2 = add2(s2, e[i]);
-      s3 = add2(s3, e[i + 1]);
+    for (int u = 0; u < U; ++u) {
+      if (!here || !units.seen(r, u)) continue;
+      exp_minus<H>(e[u], base);
+#pragma unroll
+      for (int j = 0; j < H; j += 2) {
+        s2 = add2(s2, e[u][j]);
+        s3 = add2(s3, e[u][j + 1]);
+      }
     }
     float s = sum2(add2(s2, s3));
 #pragma unroll
@@ -367,19 +389,20 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
         sum = __fmaf_rn(sh.v[parity][k][1], ex2_approx((sh.v[parity][k][0] - top) * kLog2e), sum);
       factor = ex2_approx((m - top) * kLog2e);
     }
-    factor = sum == 0.0f ? 0.0f : factor * __frcp_rn(sum);
+    factor = sum == 0.0f ? 0.0f : factor * rcp_approx(sum);
     if (!two && on) fetch(ring);
     if (!here) continue;
-    if (t.tid == 0 && t.rank == 0) a.lse[r.index] = sum == 0.0f ? kNegInf : top + logf(sum);
+    if (t.tid == 0 && t.rank == 0) a.lse[this_index] = sum == 0.0f ? kNegInf : __fmaf_rn(lg2_approx(sum), kLn2, top);
     const uint64_t by = both(kDrop ? factor * run.scale : factor);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint64_t* x = e + u * H;
-      if (r.seen(u)) {
+      uint4 o = make_uint4(0u, 0u, 0u, 0u);
+      if (units.seen(r, u)) {
+        uint64_t* x = e[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], by);
         if constexpr (kDrop) {
-          const uint64_t i[1] = {r.offset(u) / dtype_bytes(T)};
+          const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
           bool keep[V];
           drop_keep<1, V>(run, i, keep);
 #pragma unroll
@@ -389,25 +412,22 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
             x[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
           }
         }
-        r.mask(u, 0.0f, x);  // a row with a NaN has a NaN factor
-      } else {
-#pragma unroll
-        for (int j = 0; j < H; ++j) x[j] = 0;
+        units.mask(r, u, 0.0f, x);  // a row with a NaN has a NaN factor
+        o = act_narrow2<T>(x);
       }
-      r.store(a, u, x);
+      units.store(a, r, u, o);
     }
   }
 }
 
-template <int T, int E, bool kDrop>
+template <int T, int E, bool kDrop, bool kEven>
 __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
-  constexpr int V = act_vec<T>(), U = E / V, P = E / 2, H = V / 2;
+  constexpr int V = act_vec<T>(), U = E / V, H = V / 2;
   extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<1> sh;
   __shared__ float ends[2][kTeamThreads / 32];
   const Team t = team_of(a.shape.warp_teams);
   const Window<V> win(a);
-  Rows<T> rows(a, t);
   const int teams = a.shape.warp_teams ? int(blockDim.x / t.threads) : 1;
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * 2 * row_words<T, E>() * blockDim.x);
@@ -415,21 +435,23 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   const uint32_t lut_at = shared_address(lut),
                  mine = shared_address(sums + (a.shape.warp_teams ? int(threadIdx.x / t.threads) : 0) * win.words());
   const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
+  const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
-  RowView<T> row;
+  Rows<T, kEven> rows(a, t, U);
+  RowView row{};
   float row_lse = 0.0f;
   auto fetch = [&](uint32_t slot) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      row.fetch(a, a.s, bytes, u, slot + uint32_t(2 * u) * pitch);
-      row.fetch(a, a.dp, bytes, u, slot + uint32_t(2 * u + 1) * pitch);
+      units.fetch(a, a.s, bytes, row, u, slot + uint32_t(2 * u) * pitch);
+      units.fetch(a, a.dp, bytes, row, u, slot + uint32_t(2 * u + 1) * pitch);
     }
-    row_lse = __ldg(a.lse_in + row.index);
   };
-  rows.start();
-  if (rows.left) {
-    row = RowView<T>(rows, t, U);
+  bool on = rows.left > 0;
+  if (on) {
+    row = units.view(a, rows);
+    row_lse = __ldg(a.lse_in + rows.index);
     fetch(ring);
   }
   copy_async_commit();
@@ -442,59 +464,50 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   const uint64_t scale = both(a.scale);
   const float drop_scale = kDrop ? run.scale : 1.0f;
   float left = 0.0f, right = 0.0f;  // dl of units wholly at rel <= -W, or at rel >= hi
-  bool on = rows.left > 0;
   const bool two = a.ring_rows == 2;
   for (uint32_t turn = 0; __any_sync(0xffffffffu, on); ++turn) {
     const uint32_t slot = ring + (two ? turn & 1u : 0u) * (uint32_t(2 * U) * pitch);
-    const RowView<T> r = row;
+    const RowView r = row;
     const bool here = on;
-    const float lse = row_lse, base = lse == kNegInf ? 0.0f : lse;  // all logits are -inf then, and every P is 0
+    const float base = row_lse == kNegInf ? 0.0f : row_lse;  // all logits are -inf then, and every P is 0
     if (on) {
-      rows.next();
+      rows.next(a);
       on = rows.left > 0;
       if (on) {
-        row = RowView<T>(rows, t, U);
+        row = units.view(a, rows);
+        row_lse = __ldg(a.lse_in + rows.index);
         if (two) fetch(ring + ((turn & 1u) ^ 1u) * (uint32_t(2 * U) * pitch));
       }
     }
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
-    uint64_t p[P], d[P];
+    uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint64_t *x = p + u * H, *y = d + u * H;
-      if (here && r.seen(u)) {
-        act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), x);
-        act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), y);
-        r.logits(win, lut_at, bias_left, bias_right, scale, u, x);
-        r.mask(u, kNegInf, x);
-        r.mask(u, 0.0f, y);
-        if constexpr (kDrop) {
-          const uint64_t i[1] = {r.offset(u) / dtype_bytes(T)};
-          bool keep[V];
-          drop_keep<1, V>(run, i, keep);
-#pragma unroll
-          for (int j = 0; j < H; ++j) {
-            float lo, hi;
-            unpack2(y[j], lo, hi);
-            y[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
-          }
-        }
-      } else {
+      if (!here || !units.seen(r, u)) continue;
+      act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
+      act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
+      units.logits(r, win, lut_at, bias_left, bias_right, scale, u, p[u]);
+      units.mask(r, u, kNegInf, p[u]);
+      units.mask(r, u, 0.0f, d[u]);
+      if constexpr (kDrop) {
+        const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
+        bool keep[V];
+        drop_keep<1, V>(run, i, keep);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
-          x[j] = both(kNegInf);
-          y[j] = 0;
+          float lo, hi;
+          unpack2(d[u][j], lo, hi);
+          d[u][j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
         }
       }
-    }
-    exp_minus(p, base);
-    uint64_t s2 = mul2(p[0], d[0]), s3 = mul2(p[1], d[1]);
+      exp_minus<H>(p[u], base);
 #pragma unroll
-    for (int i = 2; i < P; i += 2) {
-      s2 = fma2(p[i], d[i], s2);
-      s3 = fma2(p[i + 1], d[i + 1], s3);
+      for (int j = 0; j < H; j += 2) {
+        s2 = fma2(p[u][j], d[u][j], s2);
+        s3 = fma2(p[u][j + 1], d[u][j + 1], s3);
+      }
     }
     float dot[1] = {sum2(add2(s2, s3))};
     team_sum<1>(t, sh, int(turn & 1u), dot);
@@ -505,12 +518,13 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint64_t *x = p + u * H, o[H];
-      if (r.seen(u)) {
+      uint4 o = make_uint4(0u, 0u, 0u, 0u);
+      if (units.seen(r, u)) {
+        uint64_t* x = p[u];
 #pragma unroll
-        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u * H + j], by, minus));
-        r.mask(u, 0.0f, x);  // a NaN sum stays with the keys that are seen
-        const int rel = r.key(u) - r.pos;
+        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
+        units.mask(r, u, 0.0f, x);  // a NaN sum stays with the keys that are seen
+        const int rel = units.key(r, u) - r.pos;
         if (rel >= win.hi || rel + V - 1 <= -win.w) {
           uint64_t v = x[0];
 #pragma unroll
@@ -529,12 +543,10 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
           }
         }
 #pragma unroll
-        for (int j = 0; j < H; ++j) o[j] = mul2(x[j], scale);
-      } else {
-#pragma unroll
-        for (int j = 0; j < H; ++j) o[j] = 0;
+        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], scale);
+        o = act_narrow2<T>(x);
       }
-      r.store(a, u, o);
+      units.store(a, r, u, o);
     }
   }
   // fold the windows by bucket
@@ -590,21 +602,23 @@ __global__ void __launch_bounds__(256) bias_table_join_kernel(const float* __res
   if (lane == 0) dtable[out] = float(v);
 }
 
-template <int T, bool kDrop>
-const void* kernel_of_type(int elems, bool grad) {
+template <int T, int E, bool kDrop>
+const void* kernel_of_fit(bool grad, bool even) {
   if (grad)
-    return elems == 8    ? (const void*)bias_softmax_grad_kernel<T, 8, kDrop>
-           : elems == 16 ? (const void*)bias_softmax_grad_kernel<T, 16, kDrop>
-                         : (const void*)bias_softmax_grad_kernel<T, 32, kDrop>;
-  return elems == 8    ? (const void*)bias_softmax_kernel<T, 8, kDrop>
-         : elems == 16 ? (const void*)bias_softmax_kernel<T, 16, kDrop>
-                       : (const void*)bias_softmax_kernel<T, 32, kDrop>;
+    return even ? (const void*)bias_softmax_grad_kernel<T, E, kDrop, true> : (const void*)bias_softmax_grad_kernel<T, E, kDrop, false>;
+  return even ? (const void*)bias_softmax_kernel<T, E, kDrop, true> : (const void*)bias_softmax_kernel<T, E, kDrop, false>;
+}
+template <int T, bool kDrop>
+const void* kernel_of_type(const BiasSoftmaxArgs& a, bool grad) {
+  const bool even = a.aligned && a.keys % uint32_t(act_vec<T>()) == 0;
+  return a.shape.elems == 8    ? kernel_of_fit<T, 8, kDrop>(grad, even)
+         : a.shape.elems == 16 ? kernel_of_fit<T, 16, kDrop>(grad, even)
+                               : kernel_of_fit<T, 32, kDrop>(grad, even);
 }
 template <bool kDrop>
 const void* kernel_of(const BiasSoftmaxArgs& a, bool grad) {
-  return a.type == kF32   ? kernel_of_type<kF32, kDrop>(a.shape.elems, grad)
-         : a.type == kF16 ? kernel_of_type<kF16, kDrop>(a.shape.elems, grad)
-                          : kernel_of_type<kBF16, kDrop>(a.shape.elems, grad);
+  return a.type == kF32   ? kernel_of_type<kF32, kDrop>(a, grad)
+         : a.type == kF16 ? kernel_of_type<kF16, kDrop>(a, grad) : kernel_of_type<kBF16, kDrop>(a, grad);
 }
 const void* kernel_for(const BiasSoftmaxArgs& a, bool grad) {
   return a.drop.on ? kernel_of<true>(a, grad) : kernel_of<false>(a, grad);
@@ -632,8 +646,19 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
     while (span > uint64_t(s.warp_teams) * uint64_t(s.elems)) s.warp_teams *= 2;
     return s;
   }
-  if (rows < uint64_t(sms) * 2) s.elems = 8;  // few rows: more threads for each
-  while (s.elems < 32 && span > uint64_t(kTeamThreads) * s.elems) s.elems *= 2;
+  // elements a thread: the least threads * (elements + 8), a row's own work
+  // being worth about 8 elements of a thread; few rows take more threads for each
+  uint64_t least = UINT64_MAX;
+  s.elems = 32;
+  for (int e : {32, 16, 8}) {
+    const uint64_t threads = (span + uint64_t(e) - 1) / uint64_t(e) + 31 & ~uint64_t(31);
+    if (threads > uint64_t(kTeamThreads)) break;
+    const uint64_t cost = rows < uint64_t(sms) * 2 ? uint64_t(e) : threads * uint64_t(e + 8);
+    if (cost < least) {
+      least = cost;
+      s.elems = e;
+    }
+  }
   // few rows: spread each over a cluster while SMs idle and every CTA keeps 256 threads' worth of a row
   while (s.ctas < kTeamCluster &&
          (span > uint64_t(kTeamThreads) * s.elems * s.ctas ||
