@@ -133,7 +133,8 @@ struct Rows {
     length = int(a.keys);
     place = 0;
     if (a.lengths) length = max(min(__ldg(a.lengths + b), length), 0);
-    if (a.offsets) place = __ldg(a.offsets + b);
+    // far positions meet only the window's ends, whatever their distance
+    if (a.offsets) place = max(min(__ldg(a.offsets + b), (1 << 30) - 1), -(1 << 30));
     index = (uint64_t(b) * a.heads + head) * a.queries + q;
   }
   __device__ __forceinline__ void next(const BiasSoftmaxArgs& a) {
@@ -155,6 +156,13 @@ struct RowView {
   uint64_t off;
   int k, visible, pos;  // keys [0, visible) are seen; position of the query
 };
+// What the units u of a warp's lanes are, bit u: some are seen, all are whole
+// and seen, some reach into the window.  Decided for the warp, so that no
+// unit costs a divergent branch: lanes without a visible key work along on what
+// their words last held, and are masked.
+struct Slots {
+  uint32_t seen, whole, near;
+};
 template <int T, bool kEven>
 struct Units {
   static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
@@ -172,11 +180,9 @@ struct Units {
       r.k -= int(shift);
     }
     r.off = e * B;
-    const int64_t at = int64_t(rows.place) + int64_t(rows.q);
+    r.pos = rows.place + int(rows.q);  // q is below 2^30
     r.visible = rows.length;
-    if (a.causal) r.visible = int(max(min(int64_t(rows.length), at + 1), int64_t(0)));
-    // far positions meet only the window's ends, whatever their distance
-    r.pos = int(max(min(at, int64_t(1) << 30), -(int64_t(1) << 30)));
+    if (a.causal) r.visible = max(min(r.visible, r.pos + 1), 0);
     return r;
   }
   __device__ __forceinline__ int key(const RowView& r, int u) const { return r.k + u * key_step; }
@@ -204,6 +210,18 @@ struct Units {
       st_shared(slot, make_uint4(w[0], w[1], w[2], w[3]));
     }
   }
+  template <int U>
+  __device__ __forceinline__ Slots slots(const RowView& r, const Window<V>& win, bool here) const {
+    Slots s{0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k0 = key(r, u), rel = k0 - r.pos;
+      s.seen |= __any_sync(0xffffffffu, here && seen(r, u)) ? 1u << u : 0u;
+      s.whole |= __all_sync(0xffffffffu, here && (kEven || k0 >= 0) && k0 + V <= r.visible) ? 1u << u : 0u;
+      s.near |= __any_sync(0xffffffffu, rel < win.hi && rel + V - 1 > -win.w) ? 1u << u : 0u;
+    }
+    return s;
+  }
   // the unit's elements that belong to the row
   __device__ __forceinline__ void store(const BiasSoftmaxArgs& a, const RowView& r, int u, const uint4& o) const {
     const int k0 = key(r, u);
@@ -224,7 +242,6 @@ struct Units {
   // v <- v where the key is visible, else `other`
   __device__ __forceinline__ void mask(const RowView& r, int u, float other, uint64_t* v) const {
     const int k0 = key(r, u);
-    if ((kEven || k0 >= 0) && k0 + V <= r.visible) return;
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       float lo, hi;
@@ -234,16 +251,17 @@ struct Units {
                        (kEven || at + 1 >= 0) && at + 1 < r.visible ? hi : other);
     }
   }
-  // x <- scale x + bias
+  // x <- scale x + bias; `near`: some lane's unit reaches into the window
   __device__ __forceinline__ void logits(const RowView& r, const Window<V>& win, uint32_t lut, float left, float right,
-                                         uint64_t scale, int u, uint64_t* x) const {
+                                         uint64_t scale, int u, bool near, uint64_t* x) const {
     const int rel = key(r, u) - r.pos;
-    if (rel >= win.hi || rel + V - 1 <= -win.w) {
+    if (!near) {
       const uint64_t bias = both(rel >= win.hi ? right : left);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) x[j] = fma2(x[j], scale, bias);
     } else {
-      const Places<V> at(lut, win.place(rel));
+      // the places from hi on, and those up to -W, hold the constants
+      const Places<V> at(lut, win.place(max(min(rel, win.hi), -win.w - (V - 1))));
 #pragma unroll
       for (int j = 0; j < V; j += 2)
         x[j / 2] = fma2(x[j / 2], scale, pack2(ld_shared_f32(at(j)), ld_shared_f32(at(j + 1))));
@@ -262,11 +280,12 @@ __device__ __forceinline__ float lg2_approx(float v) {
   return r;
 }
 
-// v <- exp(v - m); v may be -inf, m is not.
+// v <- exp(v - m); v may be -inf, m is not.  `direct`: |m| is at most 2^100 in
+// every lane.
 template <int N>
-__device__ __forceinline__ void exp_minus(uint64_t* v, float m) {
+__device__ __forceinline__ void exp_minus(uint64_t* v, float m, bool direct) {
   const uint64_t l = both(kLog2e);
-  if (fabsf(m) <= 0x1p100f) {
+  if (direct) {
     const uint64_t nm = both(-m * kLog2e);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = fma2(v[i], l, nm);
@@ -341,14 +360,15 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
+    const Slots of = units.template slots<U>(r, win, here);
     uint64_t e[U][H];
     float m = kNegInf;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!here || !units.seen(r, u)) continue;
+      if (!(of.seen >> u & 1u)) continue;
       act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), e[u]);
-      units.logits(r, win, lut_at, left, right, scale, u, e[u]);
-      units.mask(r, u, kNegInf, e[u]);
+      units.logits(r, win, lut_at, left, right, scale, u, of.near >> u & 1u, e[u]);
+      if (!(of.whole >> u & 1u)) units.mask(r, u, kNegInf, e[u]);
 #pragma unroll
       for (int j = 0; j < H; ++j) {
         float lo, hi;
@@ -360,11 +380,12 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     for (int d = 16; d; d >>= 1)
       if (uint32_t(d) < t.lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float base = m == kNegInf ? 0.0f : m;  // nothing visible: every 2^x below is 0
+    const bool direct = __all_sync(0xffffffffu, fabsf(base) <= 0x1p100f);
     uint64_t s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!here || !units.seen(r, u)) continue;
-      exp_minus<H>(e[u], base);
+      if (!(of.seen >> u & 1u)) continue;
+      exp_minus<H>(e[u], base, direct);
 #pragma unroll
       for (int j = 0; j < H; j += 2) {
         s2 = add2(s2, e[u][j]);
@@ -397,7 +418,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (units.seen(r, u)) {
+      if (of.seen >> u & 1u) {
         uint64_t* x = e[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], by);
@@ -412,7 +433,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
             x[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
           }
         }
-        units.mask(r, u, 0.0f, x);  // a row with a NaN has a NaN factor
+        if (!(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);  // a row with a NaN has a NaN factor
         o = act_narrow2<T>(x);
       }
       units.store(a, r, u, o);
@@ -482,15 +503,19 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
+    const Slots of = units.template slots<U>(r, win, here);
+    const bool direct = __all_sync(0xffffffffu, fabsf(base) <= 0x1p100f);
     uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!here || !units.seen(r, u)) continue;
+      if (!(of.seen >> u & 1u)) continue;
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
-      units.logits(r, win, lut_at, bias_left, bias_right, scale, u, p[u]);
-      units.mask(r, u, kNegInf, p[u]);
-      units.mask(r, u, 0.0f, d[u]);
+      units.logits(r, win, lut_at, bias_left, bias_right, scale, u, of.near >> u & 1u, p[u]);
+      if (!(of.whole >> u & 1u)) {
+        units.mask(r, u, kNegInf, p[u]);
+        units.mask(r, u, 0.0f, d[u]);
+      }
       if constexpr (kDrop) {
         const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
         bool keep[V];
@@ -502,7 +527,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
           d[u][j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
         }
       }
-      exp_minus<H>(p[u], base);
+      exp_minus<H>(p[u], base, direct);
 #pragma unroll
       for (int j = 0; j < H; j += 2) {
         s2 = fma2(p[u][j], d[u][j], s2);
@@ -519,13 +544,13 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (units.seen(r, u)) {
+      if (of.seen >> u & 1u) {
         uint64_t* x = p[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
-        units.mask(r, u, 0.0f, x);  // a NaN sum stays with the keys that are seen
+        if (!(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);  // a NaN sum stays with the keys that are seen
         const int rel = units.key(r, u) - r.pos;
-        if (rel >= win.hi || rel + V - 1 <= -win.w) {
+        if (!(of.near >> u & 1u) || rel >= win.hi || rel + V - 1 <= -win.w) {
           uint64_t v = x[0];
 #pragma unroll
           for (int j = 1; j < H; ++j) v = add2(v, x[j]);
