@@ -119,13 +119,16 @@ struct Rows {
 
   __device__ __forceinline__ Rows(const BiasSoftmaxArgs& a, const Team& t, int units) {
     const uint32_t cta = blockIdx.x / t.ctas, chunk = cta / a.heads;
-    const uint64_t n = a.batch * a.queries, begin = n * chunk / a.chunks, end = n * (chunk + 1) / a.chunks;
+    const uint32_t teams = a.shape.warp_teams ? blockDim.x / t.threads : 1;
     const uint32_t team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
+    // rows of one head go round its teams, so short sequences and the short rows
+    // of a causal head fall to all of them alike
+    const uint64_t n = a.batch * a.queries, begin = uint64_t(chunk) * teams + team;
     head = cta % a.heads;
-    step = a.shape.warp_teams ? blockDim.x / t.threads : 1;
-    left = begin + team < end ? uint32_t((end - begin - team + step - 1) / step) : 0;
-    b = uint32_t((begin + team) / a.queries);
-    q = uint32_t((begin + team) % a.queries);
+    step = a.chunks * teams;
+    left = begin < n ? uint32_t((n - begin + step - 1) / step) : 0;
+    b = uint32_t(begin / a.queries);
+    q = uint32_t(begin % a.queries);
     mine = (t.rank * uint32_t(units) * t.threads + t.tid) * uint32_t(V);
     if (left) sequence(a);
   }
