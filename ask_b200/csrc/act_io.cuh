@@ -141,6 +141,17 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
 __device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ uint32_t ld_shared_word(uint32_t at) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
+  return r;
+}
+__device__ __forceinline__ void st_shared_word(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void copy_word_to_shared(uint32_t at, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copy_to_shared(uint32_t at, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
 }

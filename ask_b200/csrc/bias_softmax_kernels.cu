@@ -119,13 +119,11 @@ struct Rows {
 
   __device__ __forceinline__ Rows(const BiasSoftmaxArgs& a, const Team& t, int units) {
     const uint32_t cta = blockIdx.x / t.ctas, chunk = cta / a.heads;
-    const uint32_t teams = a.shape.warp_teams ? blockDim.x / t.threads : 1;
-    const uint32_t team = a.shape.warp_teams ? threadIdx.x / t.threads : 0;
     // rows of one head go round its teams, so short sequences and the short rows
     // of a causal head fall to all of them alike
-    const uint64_t n = a.batch * a.queries, begin = uint64_t(chunk) * teams + team;
+    const uint64_t n = a.batch * a.queries, begin = uint64_t(chunk) * t.count + t.index;
     head = cta % a.heads;
-    step = a.chunks * teams;
+    step = a.chunks * t.count;
     left = begin < n ? uint32_t((n - begin + step - 1) / step) : 0;
     b = uint32_t(begin / a.queries);
     q = uint32_t(begin % a.queries);
@@ -161,8 +159,10 @@ struct RowView {
 };
 // What the units u of a warp's lanes are, bit u: some are seen, all are whole
 // and seen, some reach into the window.  Decided for the warp, so that no
-// unit costs a divergent branch: lanes without a visible key work along on what
-// their words last held, and are masked.
+// unit costs a divergent branch.  Units without a visible key are worked on all
+// the same, on what their words last held, and masked: leaving them out cost
+// more (a branch around a unit's registers took 4.6 instructions an element,
+// its arithmetic takes 9); only their random words are not drawn.
 struct Slots {
   uint32_t seen, whole, near;
 };
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   constexpr int V = act_vec<T>(), U = E / V, H = V / 2;
   extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<2> sh;
-  const Team t = team_of(a.shape.warp_teams);
+  const Team t = team_of(a.shape);
   const Window<V> win(a);
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     float m = kNegInf;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!(of.seen >> u & 1u)) continue;
       act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), e[u]);
       units.logits(r, win, lut_at, left, right, scale, u, of.near >> u & 1u, e[u]);
       if (!(of.whole >> u & 1u)) units.mask(r, u, kNegInf, e[u]);
@@ -387,7 +386,6 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     uint64_t s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!(of.seen >> u & 1u)) continue;
       exp_minus<H>(e[u], base, direct);
 #pragma unroll
       for (int j = 0; j < H; j += 2) {
@@ -450,14 +448,14 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<1> sh;
   __shared__ float ends[2][kTeamThreads / 32];
-  const Team t = team_of(a.shape.warp_teams);
+  const Team t = team_of(a.shape);
   const Window<V> win(a);
-  const int teams = a.shape.warp_teams ? int(blockDim.x / t.threads) : 1;
+  const int teams = int(t.count);
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * 2 * row_words<T, E>() * blockDim.x);
   float* const sums = lut + win.words();  // the teams' windows
   const uint32_t lut_at = shared_address(lut),
-                 mine = shared_address(sums + (a.shape.warp_teams ? int(threadIdx.x / t.threads) : 0) * win.words());
+                 mine = shared_address(sums + int(t.index) * win.words());
   const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
   const Units<T, kEven> units(a, t);
   pdl_enter();
@@ -511,7 +509,6 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!(of.seen >> u & 1u)) continue;
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
       units.logits(r, win, lut_at, bias_left, bias_right, scale, u, of.near >> u & 1u, p[u]);
@@ -519,7 +516,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
         units.mask(r, u, kNegInf, p[u]);
         units.mask(r, u, 0.0f, d[u]);
       }
-      if constexpr (kDrop) {
+      if (kDrop && (of.seen >> u & 1u)) {
         const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
         bool keep[V];
         drop_keep<1, V>(run, i, keep);
@@ -667,7 +664,7 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   const uint64_t v = type == kF32 ? 4 : 8;
   // a row that starts inside a unit spreads over one more
   const uint64_t span = keys % v ? keys + v - 1 : keys;
-  TeamShape s{0, kWarpTeamThreads, 1, 32};
+  TeamShape s{0, kWarpTeamThreads, kWarpTeamThreads, 1, 32};
   if (rows >= uint64_t(sms) * 8 && span <= 32 * 32) {
     s.elems = span <= 32 * 16 ? 16 : 32;
     s.warp_teams = 4;
@@ -693,7 +690,7 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
           (rows * s.ctas * 2 <= uint64_t(sms) && span >= uint64_t(512) * s.elems * s.ctas)))
     s.ctas *= 2;
   const uint64_t per = uint64_t(s.elems) * s.ctas;
-  s.threads = int(std::max<uint64_t>(32, ((span + per - 1) / per + 31) / 32 * 32));
+  s.threads = s.team_threads = int(std::max<uint64_t>(32, ((span + per - 1) / per + 31) / 32 * 32));
   return s;
 }
 

@@ -214,6 +214,7 @@ constexpr int kDropThreads = 256;
 struct TeamShape {
   int warp_teams;  // lanes of a warp that take a row (4 to 32), 0: the whole CTA or cluster
   int threads;     // of a CTA
+  int team_threads;  // of a row's team within a CTA, where it is whole warps
   int ctas;        // of a row's cluster (1: no cluster)
   int elems;       // row elements a thread holds
 };
@@ -243,19 +244,22 @@ struct NormArgs {
   TeamShape shape;
 };
 constexpr int kNormMaxCols = 32768;
-TeamShape norm_shape(uint64_t cols, int type);
+TeamShape norm_shape(uint64_t cols, int type, bool grad);
+// How rows lie in memory: whole 16-byte units, whole 4-byte words, or anywhere
+// (16-bit types: an odd number of columns, or a tensor that starts inside a word).
+enum NormFit { NORM_UNITS = 0, NORM_WORDS = 1, NORM_ANYWHERE = 2 };
 // Row sums the gradient keeps for each column: of B*yhat, B, du*hhat, du.
 struct NormSums {
   bool t, s, p, q;
   int count() const { return int(t) + int(s) + int(p) + int(q); }
 };
 NormSums norm_sums(const NormArgs& a);
-cudaError_t norm_occupancy(const NormArgs& a, bool grad, int* blocks_per_sm);
-// `aligned`: every row of every port starts on a 16-byte boundary.
-cudaError_t norm_launch(const NormArgs& a, bool aligned, int grid, cudaStream_t stream);
-cudaError_t norm_grad_launch(const NormArgs& a, bool aligned, cudaStream_t stream);
+cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm);
+cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm);
+cudaError_t norm_launch(const NormArgs& a, NormFit fit, int grid, cudaStream_t stream);
+cudaError_t norm_grad_launch(const NormArgs& a, NormFit fit, cudaStream_t stream);
 // Rows a CTA works on at once.
-inline int team_count(const TeamShape& s) { return s.warp_teams ? s.threads / s.warp_teams : 1; }
+inline int team_count(const TeamShape& s) { return s.threads / (s.warp_teams ? s.warp_teams : s.team_threads); }
 
 // Softmax over biased scores (bias_softmax_kernels.cu).  s, p, dp, ds are
 // [batch, heads, queries, keys] of `type`, table [buckets, heads] of

@@ -1,0 +1,197 @@
+// Block norms, forward: see norm_rows.cuh.
+#include "norm_rows.cuh"
+
+namespace askb {
+
+namespace {
+
+template <int T, int F, bool kFull>
+struct Layout {
+  static constexpr int kStage = 2 * Columns<T, F>::kArrayBytes, kParams = (kFull ? 4 : 2) * kParamBytes;
+  static constexpr int kStages = ring_stages(kStage, kParams), kBytes = kStages * kStage + kParams;
+};
+
+// Centres the row (layer norm) and gives its mean and 1 / sqrt(variance + eps).
+template <int T, int F>
+__device__ __forceinline__ void row_stats(const Team& t, const Columns<T, F>& c, TeamRecords<1>& sh_mean,
+                                          TeamRecords<1>& sh_sq, int parity, bool layer, float inv_cols, float eps,
+                                          uint64_t (&v)[kPairs], float& mean, float& rstd) {
+  mean = 0.0f;
+  if (layer) {
+    float s[1] = {total(v)};
+    team_sum<1>(t, sh_mean, parity, s);
+    mean = s[0] * inv_cols;
+    c.center(mean, v);
+  }
+  float s[1] = {dot(v, v)};
+  team_sum<1>(t, sh_sq, parity, s);
+  rstd = rsqrtf(__fmaf_rn(s[0], inv_cols, eps));
+}
+
+// kFull: layer norms or biases too; a plain rms norm drops that code.
+template <int T, int F, int kForm, bool kFull, bool kDrop>
+__global__ void __launch_bounds__(kTeamThreads) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+  using Cols = Columns<T, F>;
+  using Shape = Layout<T, F, kFull>;
+  constexpr int S = Shape::kStages, P = kPairs;
+  const bool branch = kForm == FORM_ANY ? a.branch : kForm != FORM_NORM;
+  const bool post = kForm == FORM_ANY ? a.post : kForm == FORM_BOTH;
+  const bool pre = kForm == FORM_ANY ? a.pre : true;
+  const bool factors = kForm == FORM_ANY || kForm == FORM_BOTH;
+  extern __shared__ uint4 dynamic[];
+  __shared__ TeamRecords<1> sh[kFull ? 4 : 2];
+  const Team t = team_of(a.shape);
+  const Cols col(t, a);
+  // a CTA (or cluster) has a stretch of rows, and its teams take them in turn
+  const uint32_t places = gridDim.x / t.ctas, place = blockIdx.x / t.ctas;
+  const uint64_t begin = a.rows * place / places, end = a.rows * (place + 1) / places;
+  uint64_t row = begin + t.index;
+  const uint32_t mine = row < end ? uint32_t((end - row + t.count - 1) / t.count) : 0;
+  const uint32_t turns = __shfl_sync(0xffffffffu, mine, 0);  // of the warp: its first team has the most rows
+  const float inv_cols = 1.0f / float(a.cols);
+  const uint32_t ring = Cols::ring(dynamic), array = blockDim.x * uint32_t(Cols::kArrayBytes), stage_bytes = 2 * array;
+  const uint32_t pitch = blockDim.x * 16, params = shared_address(dynamic) + S * stage_bytes + threadIdx.x * 16;
+  const ParamSlot pre_w{params, pitch}, fac{params + kElems / 4 * pitch, pitch},
+      pre_b{params + 2 * (kElems / 4) * pitch, pitch}, fac_b{params + 3 * (kElems / 4) * pitch, pitch};
+  const uint64_t bytes = a.rows * a.cols * uint64_t(Cols::B), advance = t.count * uint64_t(a.cols) * Cols::B;
+  pdl_enter();
+  team_start(t);
+  DropRun run{};
+  if constexpr (kDrop) run = drop_run(a.drop, a.seed);
+  const float scale = kDrop ? run.scale : 1.0f;
+  uint64_t off = col.offset(row);
+  auto fetch = [&](uint32_t turn, uint64_t at, uint32_t slot) {
+    if (turn < mine) {
+      col.fetch(a.x, at, bytes, slot);
+      if (branch) col.fetch(a.y, at, bytes, slot + array);
+    }
+    copy_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    col.clear(ring + s * stage_bytes);
+    col.clear(ring + s * stage_bytes + array);
+  }
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s, off + s * advance, ring + s * stage_bytes);
+  if (pre) {
+    float f[kElems];
+    col.params(a.w_pre, a.ptype, 0, 1.0f, f);
+    pre_w.write(f);
+    if constexpr (kFull) {
+      col.params(a.b_pre, a.ptype, 0, 0.0f, f);
+      pre_b.write(f);
+    }
+  }
+  uint64_t group_end = 0;  // the factors in shared memory are those of the rows before it
+  uint32_t slot = ring, free_slot = ring + (S - 1) * stage_bytes;
+  for (uint32_t turn = 0; turn < turns; ++turn, row += t.count, off += advance) {
+    const int parity = int(turn & 1u);
+    const bool on = turn < mine;
+    fetch(turn + S - 1, off + (S - 1) * advance, free_slot);
+    if (factors && branch && on && row >= group_end) {
+      // post weight, gate and the dropout's scale as one factor
+      const uint64_t group = row / a.rows_per_group;
+      group_end = (group + 1) * a.rows_per_group;
+      float g[kElems], f[kElems];
+      col.params(a.gate, a.ptype, group * a.cols, 1.0f, g);
+      col.params(a.w_post, a.ptype, 0, 1.0f, f);
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        g[e] *= scale;
+        f[e] *= g[e];
+      }
+      fac.write(f);
+      if constexpr (kFull) {
+        col.params(a.b_post, a.ptype, 0, 0.0f, f);
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) f[e] *= g[e];
+        fac_b.write(f);
+      }
+    }
+    copy_async_wait<S - 1>();
+    uint64_t h[P];
+    const bool writer = on && t.tid == 0 && t.rank == 0;
+    if (branch) {
+      uint64_t n[P];
+      col.read(slot + array, a.y, off, n);
+      if (post) {
+        float mean, rstd;
+        row_stats(t, col, sh[kFull ? 2 : 0], sh[0], parity, kFull && a.layer, inv_cols, a.eps, n, mean, rstd);
+        if (writer) {
+          if (kFull && a.layer) a.stats_post[2 * row] = mean;
+          a.stats_post[kFull && a.layer ? 2 * row + 1 : row] = rstd;
+        }
+        scale_all(n, rstd);
+      }
+      if (factors) scale_by<kFull>(n, fac, fac_b);
+      else if (kDrop) scale_all(n, scale);
+      if constexpr (kDrop) col.drop(run, off, n);
+      const uint64_t alpha = both(a.alpha);
+      col.read(slot, a.x, off, h);
+#pragma unroll
+      for (int k = 0; k < P; ++k) h[k] = fma2(alpha, h[k], n[k]);
+      col.put(t, a.h, off, on, h);
+    } else {
+      col.read(slot, a.x, off, h);
+    }
+    if (pre) {
+      float mean, rstd;
+      row_stats(t, col, sh[kFull ? 3 : 1], sh[1], parity, kFull && a.layer, inv_cols, a.eps, h, mean, rstd);
+      if (writer) {
+        if (kFull && a.layer) a.stats_pre[2 * row] = mean;
+        a.stats_pre[kFull && a.layer ? 2 * row + 1 : row] = rstd;
+      }
+      scale_all(h, rstd);
+      scale_by<kFull>(h, pre_w, pre_b);
+      col.put(t, a.u, off, on, h);
+    }
+    free_slot = slot;  // read by its own thread alone, and that is done
+    slot = slot == ring + (S - 1) * stage_bytes ? ring : slot + stage_bytes;
+  }
+}
+
+template <int T, int F, int kForm, bool kFull, bool kDrop>
+struct Pick {
+  static Chosen get(unsigned threads) {
+    return {(const void*)norm_rows_kernel<T, F, kForm, kFull, kDrop>, threads * unsigned(Layout<T, F, kFull>::kBytes)};
+  }
+};
+
+}  // namespace
+
+TeamShape norm_shape(uint64_t cols, int type, bool grad) {
+  (void)type;
+  TeamShape s{0, 256, 256, 1, kElems};
+  if (cols <= 32 * kElems) {
+    s.warp_teams = 4;
+    while (cols > uint64_t(s.warp_teams) * kElems) s.warp_teams *= 2;
+  } else {
+    while (cols > uint64_t(kTeamThreads) * kElems * s.ctas) s.ctas *= 2;
+    const uint64_t per = uint64_t(kElems) * s.ctas;
+    s.threads = s.team_threads = int((((cols + per - 1) / per) + 31) / 32 * 32);
+  }
+  // The gradient's teams share a CTA as large as the registers allow: one set
+  // of column sums leaves it.
+  if (grad && s.ctas == 1) s.threads = s.warp_teams ? kTeamThreads : kTeamThreads / s.team_threads * s.team_threads;
+  return s;
+}
+
+cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
+  const Chosen c = choose<Pick>(a, fit);
+  const cudaError_t e = allow(c);
+  if (e != cudaSuccess) return e;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);
+}
+
+cudaError_t norm_launch(const NormArgs& a, NormFit fit, int grid, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  const Chosen c = choose<Pick>(a, fit);
+  const cudaError_t e = allow(c);
+  if (e != cudaSuccess) return e;
+  NormArgs args = a;
+  void* params[] = {&args};
+  return launch_rows(c.kernel, a.shape, unsigned(grid), c.shared_bytes, params, stream);
+}
+
+}  // namespace askb

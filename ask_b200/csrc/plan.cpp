@@ -931,6 +931,12 @@ uint64_t chunk_count(uint64_t groups, uint64_t units, uint64_t slots) {
   return best;
 }
 
+// The fit of a step's rows: `low` holds the low bits of every row port's address.
+NormFit norm_fit(const NormArgs& a, uint64_t low) {
+  const uint64_t bytes = a.cols * uint64_t(dtype_bytes(a.type)) | low;
+  return bytes % 16 == 0 ? NORM_UNITS : bytes % 4 == 0 ? NORM_WORDS : NORM_ANYWHERE;
+}
+
 // {"family": "block_norm" | "block_norm_grad", "dtype", "rows", "cols", "norm":
 // "rms" | "layer", "eps", "branch", "post", "pre", "bias", "gate_groups",
 // "residual_scale", "dropout", "stream_id", "param_dtype"}.  Ports that a step's
@@ -1011,10 +1017,13 @@ void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
   }
   in(a.drop.on, kI64, 2);
 
-  a.shape = norm_shape(cols, a.type);
+  a.shape = norm_shape(cols, a.type, grad);
   pl.block = a.shape.threads;
   int occ = 2;
-  if (pl.device >= 0) check_cuda(norm_occupancy(a, grad, &occ), "occupancy");
+  if (pl.device >= 0) {
+    const NormFit fit = norm_fit(a, 0);
+    check_cuda(grad ? norm_grad_occupancy(a, fit, &occ) : norm_occupancy(a, fit, &occ), "occupancy");
+  }
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
   const uint64_t teams = uint64_t(team_count(a.shape));
@@ -1366,17 +1375,22 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
     case FAM_BLOCK_NORM_GRAD: {
       NormArgs a = pl.norm;
       const uint64_t* at = ports;
-      const uint64_t vec = a.type == kF32 ? 4 : 8;
-      bool wide = a.cols % vec == 0;
-      auto in = [&](bool on, const void*& p, bool row = true) {
+      uint64_t low = 0;  // low address bits of the row ports
+      auto in = [&](bool on, const void*& p) {
         if (!on) return;
-        if (row) wide &= aligned16(*at);
+        low |= *at;
+        p = reinterpret_cast<const void*>(*at++);
+      };
+      // parameters are read in 16 bytes only beside whole units
+      auto par = [&](bool on, const void*& p) {
+        if (!on) return;
+        if (!aligned16(*at)) low |= 4;
         p = reinterpret_cast<const void*>(*at++);
       };
       auto stats = [&](bool on, const float*& p) { if (on) p = reinterpret_cast<const float*>(*at++); };
       auto out = [&](bool on, void*& p) {
         if (!on) return;
-        wide &= aligned16(*at);
+        low |= *at;
         p = reinterpret_cast<void*>(*at++);
       };
       auto out32 = [&](bool on, float*& p) { if (on) p = reinterpret_cast<float*>(*at++); };
@@ -1384,27 +1398,27 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
       if (pl.family == FAM_BLOCK_NORM) {
         in(true, a.x);
         in(a.branch, a.y);
-        in(a.post, a.w_post);
-        in(post_bias, a.b_post);
-        in(a.gated, a.gate);
-        in(a.pre, a.w_pre);
-        in(pre_bias, a.b_pre);
+        par(a.post, a.w_post);
+        par(post_bias, a.b_post);
+        par(a.gated, a.gate);
+        par(a.pre, a.w_pre);
+        par(pre_bias, a.b_pre);
         if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
         out(a.branch, a.h);
         out(a.pre, a.u);
         out32(a.post, a.stats_post);
         out32(a.pre, a.stats_pre);
-        check_cuda(norm_launch(a, wide, pl.grid, st), "block_norm launch");
+        check_cuda(norm_launch(a, norm_fit(a, low), pl.grid, st), "block_norm launch");
         break;
       }
       in(a.branch, a.dh);
       in(a.pre, a.du);
       in(a.pre, a.h_in);
       in(a.post || a.gated, a.y);
-      in(a.post, a.w_post);
-      in(post_bias && a.gated, a.b_post);
-      in(a.gated, a.gate);
-      in(a.pre, a.w_pre);
+      par(a.post, a.w_post);
+      par(post_bias && a.gated, a.b_post);
+      par(a.gated, a.gate);
+      par(a.pre, a.w_pre);
       stats(a.post, a.stats_post_in);
       stats(a.pre, a.stats_pre_in);
       if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
@@ -1418,7 +1432,7 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
       if (pl.scratch && !scratch) fail(ASK_B200_E_INVALID, "this plan needs scratch memory");
       if (scratch && !aligned16(scratch)) fail(ASK_B200_E_INVALID, "scratch must be 16-byte aligned");
       a.partial = reinterpret_cast<float*>(scratch);
-      check_cuda(norm_grad_launch(a, wide, st), "block_norm_grad launch");
+      check_cuda(norm_grad_launch(a, norm_fit(a, low), st), "block_norm_grad launch");
       break;
     }
     case FAM_BIAS_SOFTMAX:

@@ -1,9 +1,9 @@
 // The threads that share a row, and their reductions.
 //
 // A row is held by part of a warp or a warp (short rows: several independent
-// teams in a CTA, no barrier), by a CTA, or by a cluster of up to eight CTAs
-// (rows longer than a CTA's registers hold, or so few rows that most SMs would
-// idle).  A reduction
+// teams in a CTA, no barrier), by some warps or all of a CTA (a named barrier
+// for each team), or by a cluster of up to eight CTAs (rows longer than a CTA's
+// registers hold, or so few rows that most SMs would idle).  A reduction
 // folds each warp by shuffles, then every warp writes its record into the
 // shared memory of every CTA of the team (distributed shared memory within a
 // cluster), one barrier follows, and every thread folds the records in warp
@@ -33,6 +33,7 @@ struct Team {
   uint32_t lanes;    // lanes of a warp that belong to one team
   uint32_t lane, warp, warps;
   uint32_t ctas, rank;  // CTAs of the team (the cluster) and this one's place among them
+  uint32_t count, index;  // teams of this CTA, and which this is
 };
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -56,24 +57,27 @@ __device__ __forceinline__ uint32_t peer_address(const void* mine, uint32_t rank
   return r;
 }
 
-// `warp_teams`: the lanes of a team within a warp (4 to 32, a power of two), or
-// 0 where the CTA or the cluster is the team.
-__device__ __forceinline__ Team team_of(int warp_teams) {
+__device__ __forceinline__ Team team_of(const TeamShape& s) {
   Team t;
   t.lane = threadIdx.x & 31u;
-  t.lanes = warp_teams ? uint32_t(warp_teams) : 32u;
-  if (warp_teams) {
+  if (s.warp_teams) {
+    t.lanes = uint32_t(s.warp_teams);
     t.tid = t.lane & (t.lanes - 1);
     t.threads = t.lanes;
     t.warp = 0;
     t.warps = 1;
     t.ctas = 1;
     t.rank = 0;
+    t.count = blockDim.x / t.lanes;
+    t.index = threadIdx.x / t.lanes;
   } else {
-    t.tid = threadIdx.x;
-    t.threads = blockDim.x;
-    t.warp = threadIdx.x >> 5;
-    t.warps = blockDim.x >> 5;
+    t.lanes = 32;
+    t.threads = uint32_t(s.team_threads);
+    t.count = blockDim.x / t.threads;
+    t.index = t.count == 1 ? 0 : threadIdx.x / t.threads;
+    t.tid = threadIdx.x - t.index * t.threads;
+    t.warp = t.tid >> 5;
+    t.warps = t.threads >> 5;
     t.ctas = cluster_size();
     t.rank = cluster_rank();
   }
@@ -91,15 +95,19 @@ struct alignas(16) TeamRecords {
   float v[2][kTeamRecords][N];
 };
 
+// Where a team's records begin: teams that share a CTA have theirs side by side.
+__device__ __forceinline__ uint32_t team_base(const Team& t) { return t.index * t.warps; }
+
 // Write this warp's record (v, the same in all lanes) to the team; then barrier.
 template <int N>
 __device__ __forceinline__ void team_exchange(const Team& t, TeamRecords<N>& sh, int parity, const float (&v)[N]) {
   if (t.ctas == 1) {
     if (t.lane == 0) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) sh.v[parity][t.warp][n] = v[n];
+      for (int n = 0; n < N; ++n) sh.v[parity][team_base(t) + t.warp][n] = v[n];
     }
-    __syncthreads();
+    if (t.count == 1) __syncthreads();
+    else asm volatile("barrier.sync %0, %1;" ::"r"(t.index + 1u), "r"(t.threads) : "memory");
     return;
   }
   if (t.lane < t.ctas) {
@@ -123,26 +131,27 @@ __device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int 
   const uint32_t records = t.warps * t.ctas;
   if (records == 1) return;
   team_exchange<N>(t, sh, parity, v);
+  const float(*const rec)[N] = sh.v[parity] + team_base(t);
   if (records == 8) {  // rows of 4096: no loop
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       float r[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = sh.v[parity][k][n];
+      for (int k = 0; k < 8; ++k) r[k] = rec[k][n];
       v[n] = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
     }
   } else if (records < 8) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = sh.v[parity][0][n];
+    for (int n = 0; n < N; ++n) v[n] = rec[0][n];
     for (uint32_t k = 1; k < records; ++k) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) v[n] += sh.v[parity][k][n];
+      for (int n = 0; n < N; ++n) v[n] += rec[k][n];
     }
   } else {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       v[n] = 0.0f;
-      for (uint32_t k = t.lane; k < records; k += 32) v[n] += sh.v[parity][k][n];
+      for (uint32_t k = t.lane; k < records; k += 32) v[n] += rec[k][n];
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
