@@ -194,13 +194,13 @@ struct Units {
     return key(r, u) < r.visible && (kEven || key(r, u) > -V);
   }
 
-  __device__ __forceinline__ void fetch(const BiasSoftmaxArgs& a, const void* p, uint64_t bytes, const RowView& r, int u,
-                                        uint32_t slot) const {
+  // `units` lie in the tensor whole: all rows but its last one's, of an aligned tensor
+  __device__ __forceinline__ void fetch(const void* p, const RowView& r, bool units, int u, uint32_t slot) const {
     if (!seen(r, u)) return;
     const char* from = static_cast<const char*>(p) + offset(r, u);
-    if (kEven || (a.aligned && offset(r, u) + 16 <= bytes)) {
+    if (kEven || units) {
       copy_to_shared(slot, from);
-    } else {  // a tensor's last unit, or a tensor that starts inside 16 bytes: by elements
+    } else {  // by elements
       uint32_t w[4] = {};
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -232,26 +232,34 @@ struct Units {
     char* to = static_cast<char*>(a.out) + offset(r, u);
     if (kEven || (a.aligned && k0 >= 0 && k0 + V <= keys)) {
       st_stream_v4(to, o);
-    } else {
-      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+      return;
+    }
+    const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+    const int first = max(-k0, 0), end = min(keys - k0, V);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (k0 + j < 0 || k0 + j >= keys) continue;
-        if constexpr (B == 4) reinterpret_cast<uint32_t*>(to)[j] = w[j];
-        else reinterpret_cast<uint16_t*>(to)[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));
+    for (int k = 0; k < 4; ++k) {  // by words, and by halves of them
+      if constexpr (B == 4) {
+        if (k >= first && k < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+      } else {
+        const bool lo = 2 * k >= first && 2 * k < end, hi = 2 * k + 1 >= first && 2 * k + 1 < end;
+        if (lo && hi && a.aligned) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+        else {
+          if (lo) reinterpret_cast<uint16_t*>(to)[2 * k] = uint16_t(w[k]);
+          if (hi) reinterpret_cast<uint16_t*>(to)[2 * k + 1] = uint16_t(w[k] >> 16);
+        }
       }
     }
   }
   // v <- v where the key is visible, else `other`
   __device__ __forceinline__ void mask(const RowView& r, int u, float other, uint64_t* v) const {
-    const int k0 = key(r, u);
+    // key k0 + j is visible when j - first is below n, without a sign
+    const int k0 = key(r, u), first = kEven ? 0 : max(-k0, 0);
+    const uint32_t n = uint32_t(max(r.visible - k0 - first, 0));
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       float lo, hi;
       unpack2(v[j / 2], lo, hi);
-      const int at = k0 + j;
-      v[j / 2] = pack2((kEven || at >= 0) && at < r.visible ? lo : other,
-                       (kEven || at + 1 >= 0) && at + 1 < r.visible ? hi : other);
+      v[j / 2] = pack2(uint32_t(j - first) < n ? lo : other, uint32_t(j + 1 - first) < n ? hi : other);
     }
   }
   // x <- scale x + bias; `near`: some lane's unit reaches into the window
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
   const uint32_t lut_at = shared_address(lut);
-  const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
+  const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   uint64_t index = 0;
   auto fetch = [&](uint32_t slot) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) units.fetch(a, a.s, bytes, row, u, slot + uint32_t(u) * pitch);
+    for (int u = 0; u < U; ++u) units.fetch(a.s, row, a.aligned && rows.index != last_row, u, slot + uint32_t(u) * pitch);
   };
   bool on = rows.left > 0;
   if (on) {
@@ -412,6 +420,8 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
       factor = ex2_approx((m - top) * kLog2e);
     }
     factor = sum == 0.0f ? 0.0f : factor * rcp_approx(sum);
+    // masked keys hold 0 already, unless a NaN in the row makes the factor one
+    const bool odd = __any_sync(0xffffffffu, here && !(factor >= 0.0f));
     if (!two && on) fetch(ring);
     if (!here) continue;
     if (t.tid == 0 && t.rank == 0) a.lse[this_index] = sum == 0.0f ? kNegInf : __fmaf_rn(lg2_approx(sum), kLn2, top);
@@ -434,7 +444,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
             x[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
           }
         }
-        if (!(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);  // a row with a NaN has a NaN factor
+        if (odd && !(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);
         o = act_narrow2<T>(x);
       }
       units.store(a, r, u, o);
@@ -456,7 +466,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   float* const sums = lut + win.words();  // the teams' windows
   const uint32_t lut_at = shared_address(lut),
                  mine = shared_address(sums + int(t.index) * win.words());
-  const uint64_t bytes = a.batch * a.heads * a.queries * a.keys * uint64_t(dtype_bytes(T));
+  const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
@@ -464,10 +474,11 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   RowView row{};
   float row_lse = 0.0f;
   auto fetch = [&](uint32_t slot) {
+    const bool whole = a.aligned && rows.index != last_row;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      units.fetch(a, a.s, bytes, row, u, slot + uint32_t(2 * u) * pitch);
-      units.fetch(a, a.dp, bytes, row, u, slot + uint32_t(2 * u + 1) * pitch);
+      units.fetch(a.s, row, whole, u, slot + uint32_t(2 * u) * pitch);
+      units.fetch(a.dp, row, whole, u, slot + uint32_t(2 * u + 1) * pitch);
     }
   };
   bool on = rows.left > 0;
@@ -537,6 +548,8 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     float dot[1] = {sum2(add2(s2, s3))};
     team_sum<1>(t, sh, int(turn & 1u), dot);
     if (a.shape.warp_teams) __syncwarp();  // the lanes' adds of the row before are done
+    // masked keys hold P = 0 already, unless the sum is a NaN or infinite
+    const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
     if (!two && on) fetch(ring);
     if (!here) continue;
     // dl = P (D(dp) - sum): the dropout's scale enters here
@@ -548,7 +561,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
         uint64_t* x = p[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
-        if (!(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);  // a NaN sum stays with the keys that are seen
+        if (odd && !(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);
         const int rel = units.key(r, u) - r.pos;
         if (!(of.near >> u & 1u) || rel >= win.hi || rel + V - 1 <= -win.w) {
           uint64_t v = x[0];
@@ -638,7 +651,8 @@ const void* kernel_of_type(const BiasSoftmaxArgs& a, bool grad) {
   const bool even = a.aligned && a.keys % uint32_t(act_vec<T>()) == 0;
   return a.shape.elems == 8    ? kernel_of_fit<T, 8, kDrop>(grad, even)
          : a.shape.elems == 16 ? kernel_of_fit<T, 16, kDrop>(grad, even)
-                               : kernel_of_fit<T, 32, kDrop>(grad, even);
+         : a.shape.elems == 32 ? kernel_of_fit<T, 32, kDrop>(grad, even)
+                               : kernel_of_fit<T, 40, kDrop>(grad, even);
 }
 template <bool kDrop>
 const void* kernel_of(const BiasSoftmaxArgs& a, bool grad) {
@@ -647,12 +661,6 @@ const void* kernel_of(const BiasSoftmaxArgs& a, bool grad) {
 }
 const void* kernel_for(const BiasSoftmaxArgs& a, bool grad) {
   return a.drop.on ? kernel_of<true>(a, grad) : kernel_of<false>(a, grad);
-}
-
-// Shared memory above the default 48 KB (static arrays included) needs the kernel's limit raised.
-cudaError_t allow_shared(const void* kernel, uint32_t bytes) {
-  return bytes <= 32 * 1024 ? cudaSuccess
-                            : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
 
 constexpr uint32_t kSharedBytes = 216 * 1024;  // dynamic shared memory of a CTA at most
@@ -665,19 +673,27 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   // a row that starts inside a unit spreads over one more
   const uint64_t span = keys % v ? keys + v - 1 : keys;
   TeamShape s{0, kWarpTeamThreads, kWarpTeamThreads, 1, 32};
-  if (rows >= uint64_t(sms) * 8 && span <= 32 * 32) {
-    s.elems = span <= 32 * 16 ? 16 : 32;
-    s.warp_teams = 4;
-    while (span > uint64_t(s.warp_teams) * uint64_t(s.elems)) s.warp_teams *= 2;
+  // The threads a row takes and the elements of each: the least threads *
+  // (elements + 8), a row's own work being worth about 8 elements of a thread.
+  // More elements cost registers (40: 5 units of 16 bits, for rows a little over
+  // a warp's 1024), fewer leave a row's work to more threads.
+  uint64_t least = UINT64_MAX;
+  if (rows >= uint64_t(sms) * 8 && span <= 32 * 40) {
+    for (int e : {40, 32, 16}) {
+      uint64_t lanes = 4;
+      while (span > lanes * uint64_t(e)) lanes *= 2;
+      if (lanes <= 32 && lanes * uint64_t(e + 8) < least) {
+        least = lanes * uint64_t(e + 8);
+        s.elems = e;
+        s.warp_teams = int(lanes);
+      }
+    }
     return s;
   }
-  // elements a thread: the least threads * (elements + 8), a row's own work
-  // being worth about 8 elements of a thread; few rows take more threads for each
-  uint64_t least = UINT64_MAX;
-  s.elems = 32;
-  for (int e : {32, 16, 8}) {
-    const uint64_t threads = (span + uint64_t(e) - 1) / uint64_t(e) + 31 & ~uint64_t(31);
-    if (threads > uint64_t(kTeamThreads)) break;
+  // few rows take more threads for each
+  for (int e : {40, 32, 16, 8}) {
+    const uint64_t threads = ((span + uint64_t(e) - 1) / uint64_t(e) + 31) / 32 * 32;
+    if (threads > uint64_t(kTeamThreads)) continue;
     const uint64_t cost = rows < uint64_t(sms) * 2 ? uint64_t(e) : threads * uint64_t(e + 8);
     if (cost < least) {
       least = cost;
@@ -714,7 +730,7 @@ void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad) {
 
 cudaError_t bias_softmax_occupancy(const BiasSoftmaxArgs& a, bool grad, int* blocks_per_sm) {
   const void* kernel = kernel_for(a, grad);
-  const cudaError_t e = allow_shared(kernel, a.shared_bytes);
+  const cudaError_t e = prepare_rows(kernel, a.shared_bytes);
   if (e != cudaSuccess) return e;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, kernel, a.shape.threads, a.shared_bytes);
 }
@@ -723,7 +739,7 @@ cudaError_t bias_softmax_launch(const BiasSoftmaxArgs& a, bool grad, cudaStream_
   const uint64_t pairs = a.batch * a.queries;
   if (pairs && a.heads) {
     const void* kernel = kernel_for(a, grad);
-    cudaError_t e = allow_shared(kernel, a.shared_bytes);
+    cudaError_t e = prepare_rows(kernel, a.shared_bytes);
     if (e != cudaSuccess) return e;
     BiasSoftmaxArgs args = a;
     void* params[] = {&args};

@@ -268,7 +268,7 @@ inline int team_count(const TeamShape& s) { return s.threads / (s.warp_teams ? s
 constexpr int kBiasMaxThresholds = 255;
 constexpr int kBiasMaxDistance = 4096;
 constexpr uint64_t kBiasMaxKeys = 131072;
-constexpr int kBiasMaxRowPerCta = 512 * 32;  // elements of a row that one CTA's registers hold
+constexpr int kBiasMaxThreads = 512;  // of a CTA
 struct BiasSoftmaxArgs {
   const void *s, *dp, *table;
   const float* lse_in;

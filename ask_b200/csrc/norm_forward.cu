@@ -179,7 +179,7 @@ TeamShape norm_shape(uint64_t cols, int type, bool grad) {
 
 cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
   const Chosen c = choose<Pick>(a, fit);
-  const cudaError_t e = allow(c);
+  const cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
   if (e != cudaSuccess) return e;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);
 }
@@ -187,7 +187,7 @@ cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
 cudaError_t norm_launch(const NormArgs& a, NormFit fit, int grid, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
   const Chosen c = choose<Pick>(a, fit);
-  const cudaError_t e = allow(c);
+  const cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
   if (e != cudaSuccess) return e;
   NormArgs args = a;
   void* params[] = {&args};

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
       float s[N];
       s[0] = dot(du, hh);
       if constexpr (kFull) s[1] = a.layer ? total(du) : 0.0f;
-      team_sum<N>(t, sh[0], parity, s);
+      team_sum<N, true>(t, sh[0], parity, s);
       const uint64_t k2 = both(-s[0] * inv_cols);
       if (branch) {
         col.read(slot, a.dh, off, g);
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
           float s[N];
           s[0] = dot(g, yy);
           if constexpr (kFull) s[1] = a.layer ? total(g) : 0.0f;
-          team_sum<N>(t, sh[1], parity, s);
+          team_sum<N, true>(t, sh[1], parity, s);
           const uint64_t r2 = both(rstd_y), k2 = both(-s[0] * inv_cols);
 #pragma unroll
           for (int k = 0; k < P; ++k) {
@@ -194,12 +194,15 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
     free_slot = slot;
     slot = slot == ring + (S - 1) * stage_bytes ? ring : slot + stage_bytes;
   }
-  // The column sums: teams of one warp are added by shuffles, the warps or teams
-  // of a CTA one after the other in shared memory (the ring is done with).
+  // The column sums: teams of one warp are added by shuffles; the warps or teams
+  // of a CTA lay theirs side by side in shared memory (the ring is done with: it
+  // held more), and the CTA adds them in order.
   const uint64_t places = uint64_t(a.groups) * a.chunks;
-  float* const joined = reinterpret_cast<float*>(dynamic);
+  float* const laid = reinterpret_cast<float*>(dynamic);
   const uint32_t order = a.shape.warp_teams ? threadIdx.x >> 5 : t.index;
   const uint32_t holders = a.shape.warp_teams ? blockDim.x >> 5 : t.count;
+  const bool direct = !a.shape.warp_teams && holders == 1;
+  const uint32_t lane_cols = direct ? 0 : (a.cols + 3u) & ~3u;
   copy_async_wait<0>();
   __syncthreads();
   auto put = [&](const uint64_t (&pairs)[P], float by, int kind) {
@@ -207,7 +210,6 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
     Cols::unpack(pairs, v);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= by;
-    float* out = a.partial + (uint64_t(kind) * places + place) * a.cols;
     if (a.shape.warp_teams) {
 #pragma unroll
       for (int d = 16; d >= 4; d >>= 1) {
@@ -215,29 +217,24 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], d);
       }
-    } else if (holders == 1) {
+      if (t.lane >= t.lanes) return;
+    }
+    float* const to = direct ? a.partial + (uint64_t(kind) * places + place) * a.cols
+                             : laid + (uint32_t(kind) * holders + order) * lane_cols;
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
+    for (int q = 0; q < Q; ++q) {
+      if (V % 4 == 0 && F == NORM_UNITS && (!direct || a.cols % 4 == 0)) {
+        if (!col.in(q)) continue;
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4*>(to + col.at(q) + j) =
+              make_float4(v[q * V + j], v[q * V + j + 1], v[q * V + j + 2], v[q * V + j + 3]);
+      } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (j < col.count(q)) out[col.at(q) + j] = v[q * V + j];
-      return;
-    }
-    for (uint32_t w = 0; w < holders; ++w) {
-      if (order == w && t.lane < t.lanes) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (j < col.count(q)) {
-              float* at = joined + col.at(q) + j;
-              *at = w ? *at + v[q * V + j] : v[q * V + j];
-            }
+          if (j < col.count(q)) to[col.at(q) + j] = v[q * V + j];
       }
-      __syncthreads();
     }
-    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) out[c] = joined[c];
-    __syncthreads();
   };
   int kind = 0;
   if (kinds.t) put(acc_t, scale, kind++);
@@ -248,89 +245,82 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
   if constexpr (kFull) {
     if (kinds.q) put(acc_q, 1.0f, kind++);
   }
+  if (direct) return;
+  __syncthreads();
+  for (int k = 0; k < kind; ++k)
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      const float* from = laid + uint32_t(k) * holders * lane_cols + c;
+      float v = from[0];
+      for (uint32_t w = 1; w < holders; ++w) v += from[w * lane_cols];
+      a.partial[(uint64_t(k) * places + place) * a.cols + c] = v;
+    }
 }
 
-// Join of the partial column sums in place order: 32 columns a CTA, 32 warps
-// sharing the places of a group (few groups) or the groups (many).
-constexpr int kJoinWarps = 32;
-constexpr uint32_t kJoinFewGroups = 32;
+// Join of the places' column sums, 32 columns a CTA, its warps sharing the places
+// and adding what they found in warp order.  A CTA row (blockIdx.y) has one task:
+// a group's gate gradient, the post norm's parameters (gate times the groups'
+// sums), or the pre norm's.
+constexpr int kJoinWarps = 16;
 
-__global__ void __launch_bounds__(32 * kJoinWarps) norm_grad_join_kernel(const NormArgs a, const NormSums kinds) {
-  __shared__ float red[2][kJoinWarps][33];
+__global__ void __launch_bounds__(32 * kJoinWarps) norm_grad_join_kernel(const __grid_constant__ NormArgs a,
+                                                                         const NormSums kinds, const uint32_t gate_rows) {
+  __shared__ float red[2][kJoinWarps][32];
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   const uint64_t c = uint64_t(blockIdx.x) * 32 + lane;
   const bool in = c < a.cols;
   const uint64_t places = uint64_t(a.groups) * a.chunks;
   pdl_enter();
-  const float* sum_t = a.partial;
-  const float* sum_s = a.partial + uint64_t(kinds.t) * places * a.cols;
-  const float* sum_p = a.partial + uint64_t(int(kinds.t) + int(kinds.s)) * places * a.cols;
-  const float* sum_q = sum_p + uint64_t(kinds.p) * places * a.cols;
-  // sum over `n` places from `first`, every `by`-th
-  auto gather = [&](const float* s, uint64_t first, uint64_t n, uint64_t begin, uint64_t by) {
-    float v = 0.0f;
-    if (in) {
-#pragma unroll 4
-      for (uint64_t k = begin; k < n; k += by) v += s[(first + k) * a.cols + c];
-    }
-    return v;
-  };
-  // over the warps, in order; the total in every warp's lane
-  auto across = [&](float x, float y, float& sx, float& sy) {
-    red[0][warp][lane] = x;
-    red[1][warp][lane] = y;
-    __syncthreads();
-    sx = sy = 0.0f;
-    for (int w = 0; w < kJoinWarps; ++w) {
-      sx += red[0][w][lane];
-      sy += red[1][w][lane];
-    }
-    __syncthreads();
-  };
-  auto param = [&](const void* p, uint64_t i) {
-    float v[1] = {0.0f};
+  const float* const sum_t = a.partial + c;
+  const float* const sum_s = sum_t + uint64_t(kinds.t) * places * a.cols;
+  const float* const sum_p = sum_s + uint64_t(kinds.s) * places * a.cols;
+  const float* const sum_q = sum_p + uint64_t(kinds.p) * places * a.cols;
+  auto param = [&](const void* p, uint64_t i, float fill) {
+    float v[1] = {fill};
     if (in && p) param_load<1>(p, a.ptype, i, v);
     return v[0];
   };
-  if (kinds.t) {
-    const float w = a.post ? param(a.w_post, c) : 1.0f;
-    const float b = a.post && a.bias && a.gated ? param(a.b_post, c) : 0.0f;
-    float dw = 0.0f, db = 0.0f;
-    auto group_out = [&](uint64_t g, float st, float ss) {
-      const float gate = a.gated ? param(a.gate, g * a.cols + c) : 1.0f;
-      dw = __fmaf_rn(gate, st, dw);
-      db = __fmaf_rn(gate, ss, db);
-      return __fmaf_rn(w, st, b * ss);
-    };
-    if (a.groups <= kJoinFewGroups) {
-      for (uint64_t g = 0; g < a.groups; ++g) {
-        float st, ss;
-        across(gather(sum_t, g * a.chunks, a.chunks, warp, kJoinWarps),
-               kinds.s ? gather(sum_s, g * a.chunks, a.chunks, warp, kJoinWarps) : 0.0f, st, ss);
-        const float dg = group_out(g, st, ss);
-        if (a.gated && in && warp == 0) a.dgate[g * a.cols + c] = dg;
+  // x, y: sums over the places [first, first + n), each times its group's gate if `gated`
+  auto gather = [&](const float* s, const float* s2, uint64_t first, uint64_t n, bool gated, float& x, float& y) {
+    float u = 0.0f, v = 0.0f;
+    if (in) {
+#pragma unroll 4
+      for (uint64_t k = first + warp; k < first + n; k += kJoinWarps) {
+        const float g = gated ? param(a.gate, k / a.chunks * a.cols + c, 1.0f) : 1.0f;
+        u = __fmaf_rn(g, s[k * a.cols], u);
+        if (s2) v = __fmaf_rn(g, s2[k * a.cols], v);
       }
-    } else {
-      for (uint64_t g = warp; g < a.groups; g += kJoinWarps) {
-        const float st = gather(sum_t, g * a.chunks, a.chunks, 0, 1);
-        const float ss = kinds.s ? gather(sum_s, g * a.chunks, a.chunks, 0, 1) : 0.0f;
-        const float dg = group_out(g, st, ss);
-        if (a.gated && in) a.dgate[g * a.cols + c] = dg;
+    }
+    red[0][warp][lane] = u;
+    red[1][warp][lane] = v;
+    __syncthreads();
+    x = y = 0.0f;
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        x += red[0][w][lane];
+        y += red[1][w][lane];
       }
-      across(dw, db, dw, db);
     }
-    if (a.post && in && warp == 0) {
-      a.dw_post[c] = dw;
-      if (a.bias) a.db_post[c] = db;
+    __syncthreads();
+  };
+  float x, y;
+  if (blockIdx.y < gate_rows) {
+    const float w = a.post ? param(a.w_post, c, 1.0f) : 1.0f, b = kinds.s ? param(a.b_post, c, 0.0f) : 0.0f;
+    for (uint64_t g = blockIdx.y; g < a.groups; g += gate_rows) {
+      gather(sum_t, kinds.s ? sum_s : nullptr, g * a.chunks, a.chunks, false, x, y);
+      if (in && warp == 0) a.dgate[g * a.cols + c] = __fmaf_rn(w, x, b * y);
     }
-  }
-  if (kinds.p) {
-    float sp, sq;
-    across(gather(sum_p, 0, places, warp, kJoinWarps), kinds.q ? gather(sum_q, 0, places, warp, kJoinWarps) : 0.0f, sp,
-           sq);
+  } else if (blockIdx.y == gate_rows && a.post) {
+    gather(sum_t, kinds.s ? sum_s : nullptr, 0, places, a.gated, x, y);
     if (in && warp == 0) {
-      a.dw_pre[c] = sp;
-      if (a.bias) a.db_pre[c] = sq;
+      a.dw_post[c] = x;
+      if (a.bias) a.db_post[c] = y;
+    }
+  } else {
+    gather(sum_p, kinds.q ? sum_q : nullptr, 0, places, false, x, y);
+    if (in && warp == 0) {
+      a.dw_pre[c] = x;
+      if (a.bias) a.db_pre[c] = y;
     }
   }
 }
@@ -350,7 +340,7 @@ NormSums norm_sums(const NormArgs& a) {
 
 cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
   const Chosen c = choose<Pick>(a, fit);
-  const cudaError_t e = allow(c);
+  const cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
   if (e != cudaSuccess) return e;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);
 }
@@ -360,7 +350,7 @@ cudaError_t norm_grad_launch(const NormArgs& a, NormFit fit, cudaStream_t stream
   NormSums kinds = norm_sums(a);
   if (a.rows) {
     const Chosen c = choose<Pick>(a, fit);
-    cudaError_t e = allow(c);
+    cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
     if (e != cudaSuccess) return e;
     void* params[] = {&args, &kinds};
     e = launch_rows(c.kernel, a.shape, a.groups * a.chunks * unsigned(a.shape.ctas), c.shared_bytes, params, stream);
@@ -369,7 +359,9 @@ cudaError_t norm_grad_launch(const NormArgs& a, NormFit fit, cudaStream_t stream
     args.chunks = 0;  // the column sums of no rows are zero
   }
   if (kinds.count() == 0) return cudaSuccess;
-  (void)launch_pdl(&norm_grad_join_kernel, dim3((a.cols + 31) / 32), dim3(32 * kJoinWarps), stream, args, kinds);
+  const uint32_t gate_rows = a.gated ? std::min<uint32_t>(a.groups, 1024) : 0;
+  (void)launch_pdl(&norm_grad_join_kernel, dim3((a.cols + 31) / 32, gate_rows + (a.post ? 1u : 0u) + (a.pre ? 1u : 0u)),
+                   dim3(32 * kJoinWarps), stream, args, kinds, gate_rows);
   return cudaGetLastError();
 }
 

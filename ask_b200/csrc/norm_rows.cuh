@@ -295,12 +295,6 @@ struct Chosen {
   const void* kernel;
   unsigned shared_bytes;
 };
-// Dynamic shared memory above 32 KB (48 KB with the static part) has to be asked for.
-inline cudaError_t allow(const Chosen& c) {
-  return c.shared_bytes <= 32 * 1024
-             ? cudaSuccess
-             : cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(c.shared_bytes));
-}
 inline int norm_form(const NormArgs& a) {
   if (!a.branch) return FORM_NORM;
   if (a.post && a.pre) return FORM_BOTH;

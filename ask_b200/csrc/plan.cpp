@@ -1103,7 +1103,7 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
 
   a.aligned = 1;  // until a launch sees the addresses
   a.shape = bias_softmax_shape(keys, rows, a.type, grad, pl.num_sms);
-  if (a.shape.threads * a.shape.elems > kBiasMaxRowPerCta)
+  if (a.shape.threads > kBiasMaxThreads)
     fail(ASK_B200_E_UNSUPPORTED, "rows that start inside a 16-byte unit take at most " +
                                      std::to_string(kBiasMaxKeys - 7) + " keys");
   bias_softmax_shared(&a, grad);

@@ -19,6 +19,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "kernels.h"
 
 namespace askb {
@@ -99,14 +103,18 @@ struct alignas(16) TeamRecords {
 __device__ __forceinline__ uint32_t team_base(const Team& t) { return t.index * t.warps; }
 
 // Write this warp's record (v, the same in all lanes) to the team; then barrier.
-template <int N>
+// kShared: several teams of whole warps may share the CTA, each with its named
+// barrier.  Such a kernel reserves all 16 barriers of a CTA, and an SM then
+// holds 4 CTAs at most (65536 norm rows of 1024 took 175 us so, and 124 without), so
+// only a kernel whose CTAs fill the SM asks for it.
+template <int N, bool kShared = false>
 __device__ __forceinline__ void team_exchange(const Team& t, TeamRecords<N>& sh, int parity, const float (&v)[N]) {
   if (t.ctas == 1) {
     if (t.lane == 0) {
 #pragma unroll
       for (int n = 0; n < N; ++n) sh.v[parity][team_base(t) + t.warp][n] = v[n];
     }
-    if (t.count == 1) __syncthreads();
+    if (!kShared || t.count == 1) __syncthreads();
     else asm volatile("barrier.sync %0, %1;" ::"r"(t.index + 1u), "r"(t.threads) : "memory");
     return;
   }
@@ -120,7 +128,7 @@ __device__ __forceinline__ void team_exchange(const Team& t, TeamRecords<N>& sh,
 }
 
 // Sum of N values over the team, the same bits in every thread.
-template <int N>
+template <int N, bool kShared = false>
 __device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int parity, float (&v)[N]) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
@@ -130,7 +138,7 @@ __device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int 
   }
   const uint32_t records = t.warps * t.ctas;
   if (records == 1) return;
-  team_exchange<N>(t, sh, parity, v);
+  team_exchange<N, kShared>(t, sh, parity, v);
   const float(*const rec)[N] = sh.v[parity] + team_base(t);
   if (records == 8) {  // rows of 4096: no loop
 #pragma unroll
@@ -159,6 +167,25 @@ __device__ __forceinline__ void team_sum(const Team& t, TeamRecords<N>& sh, int 
       for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], d);
     }
   }
+}
+
+// Readies a row kernel on the current device, once: all of an SM's memory that
+// can be shared memory is to be that (by itself the driver kept back so much
+// that 4 CTAs ran where 10 fit), and a CTA may use `shared_bytes` of it.
+inline cudaError_t prepare_rows(const void* kernel, unsigned shared_bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, unsigned> ready;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  unsigned& allowed = ready[{kernel, device}];
+  if (allowed > shared_bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared_bytes));
+  if (e == cudaSuccess) allowed = shared_bytes + 1;
+  return e;
 }
 
 // Launch of a row kernel: CTAs of the shape's threads in clusters of its size,
