@@ -25,13 +25,11 @@
 // units are on their way (cp.async into words that only their own thread reads)
 // while this row is worked on.
 //
-// exp(l - m) is 2^(l L - RN(m L)) with L = log2 e: an element costs a fused
-// multiply-add for its logit, one for the exponent (both on f32 pairs) and
-// ex2.approx (relative error 2^-22).  The rounding of m L is one factor for all
-// that share m.  Where m L could overflow (|m| > 2^100: rows at the type's
-// lowest value) the difference is taken first.  Each warp takes its own
-// maximum, and its sum is rescaled when the team's records meet: one exchange a
-// row.
+// exp(l - m) is 2^((l - m) log2 e) by ex2.approx (relative error 2^-22); the
+// difference is taken first, as m log2 e overflows for rows at the type's
+// lowest value (and a branch for them cost more than the second operation).
+// Each warp takes its own maximum, and its sum is rescaled when the team's
+// records meet: one exchange a row.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -96,14 +94,57 @@ __device__ __forceinline__ int bucket_of(const BiasSoftmaxArgs& a, int rel) {
   return a.bidirectional && rel > 0 ? lo + a.n_thresholds + 1 : lo;
 }
 
-// The head's bias by distance.
+// The window as units meet it: V copies, the r-th shifted by r places, so that a
+// unit's V biases are V neighbouring words on a 16-byte boundary (2 loads in place
+// of V, and no place to work out for each).  Column c of copy r holds distances
+// V (c + low) + r and up; columns at either end hold the constants.  They pay
+// where teams have many rows and the window is not too wide.
 template <int V>
-__device__ __forceinline__ void fill_window(const BiasSoftmaxArgs& a, const Window<V>& win, uint32_t head, float* lut) {
+struct Lut {
+  uint32_t at;        // shared address of the window
+  uint32_t copies;    // of the copies
+  int columns;        // of a copy; 0: there are none
+  int low, high;      // first and last column
+  float left, right;  // biases at rel <= -W and at rel >= hi
+  __host__ __device__ static int first_column(int w) { return -((w + 2 * V - 2 + V - 1) / V); }
+  __host__ __device__ static int last_column(int hi) { return (hi + V - 1) / V; }
+  __host__ __device__ static int words(const Window<V>& win) {
+    return (last_column(win.hi) - first_column(win.w) + 1) * V * V;
+  }
+  __device__ __forceinline__ uint32_t shifted(int rel) const {
+    const int c = max(min(rel >> (V == 8 ? 3 : 2), high), low) - low;
+    return copies + uint32_t(((rel & (V - 1)) * columns + c) * (V * 4));
+  }
+};
+
+// The head's bias by distance into `window` (and the copies behind it).
+template <int V>
+__device__ __forceinline__ Lut<V> fill_window(const BiasSoftmaxArgs& a, const Window<V>& win, uint32_t head, float* window,
+                                              float* copies) {
   for (int i = int(threadIdx.x); i < win.places(); i += int(blockDim.x)) {
     float v[1];
     param_load<1>(a.table, a.table_type, uint64_t(bucket_of(a, win.rel(i))) * a.heads + head, v);
-    lut[win.word(i)] = v[0];
+    window[win.word(i)] = v[0];
   }
+  __syncthreads();
+  Lut<V> lut;
+  lut.at = shared_address(window);
+  lut.copies = shared_address(copies);
+  lut.low = Lut<V>::first_column(win.w);
+  lut.high = Lut<V>::last_column(win.hi);
+  lut.columns = a.window_copies ? lut.high - lut.low + 1 : 0;
+  lut.left = window[0];
+  lut.right = window[win.word(win.places() - 1)];
+  if (lut.columns) {
+    for (int i = int(threadIdx.x); i < lut.columns * V; i += int(blockDim.x))
+#pragma unroll
+      for (int r = 0; r < V; ++r) {
+        const int rel = V * lut.low + i + r;  // column i / V of copy r, word i % V
+        copies[r * lut.columns * V + i] = window[win.word(win.place(max(min(rel, win.hi), -win.w)))];
+      }
+    __syncthreads();
+  }
+  return lut;
 }
 
 // The rows of a team, one after the other: pairs (batch, query) of one head.
@@ -157,15 +198,12 @@ struct RowView {
   uint64_t off;
   int k, visible, pos;  // keys [0, visible) are seen; position of the query
 };
-// What the units u of a warp's lanes are, bit u: some are seen, all are whole
-// and seen, some reach into the window.  Decided for the warp, so that no
-// unit costs a divergent branch.  Units without a visible key are worked on all
-// the same, on what their words last held, and masked: leaving them out cost
-// more (a branch around a unit's registers took 4.6 instructions an element,
-// its arithmetic takes 9); only their random words are not drawn.
-struct Slots {
-  uint32_t seen, whole, near;
-};
+// What a unit of a warp's lanes is (seen by some, whole and seen in all, reaching
+// into the window in some) is decided for the warp by votes, so that no unit
+// costs a divergent branch.  Units without a visible key are worked on all the
+// same, on what their words last held, and masked: leaving them out cost more
+// (a branch around a unit's registers took 4.6 instructions an element, its
+// arithmetic takes 9); only their random words are not drawn.
 template <int T, bool kEven>
 struct Units {
   static constexpr int V = act_vec<T>(), B = dtype_bytes(T);
@@ -213,17 +251,14 @@ struct Units {
       st_shared(slot, make_uint4(w[0], w[1], w[2], w[3]));
     }
   }
-  template <int U>
-  __device__ __forceinline__ Slots slots(const RowView& r, const Window<V>& win, bool here) const {
-    Slots s{0, 0, 0};
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k0 = key(r, u), rel = k0 - r.pos;
-      s.seen |= __any_sync(0xffffffffu, here && seen(r, u)) ? 1u << u : 0u;
-      s.whole |= __all_sync(0xffffffffu, here && (kEven || k0 >= 0) && k0 + V <= r.visible) ? 1u << u : 0u;
-      s.near |= __any_sync(0xffffffffu, rel < win.hi && rel + V - 1 > -win.w) ? 1u << u : 0u;
-    }
-    return s;
+  __device__ __forceinline__ bool any_seen(const RowView& r, int u) const { return __any_sync(0xffffffffu, seen(r, u)); }
+  __device__ __forceinline__ bool all_whole(const RowView& r, int u) const {
+    const int k0 = key(r, u);
+    return __all_sync(0xffffffffu, (kEven || k0 >= 0) && k0 + V <= r.visible);
+  }
+  __device__ __forceinline__ bool any_near(const RowView& r, const Window<V>& win, int u) const {
+    const int rel = key(r, u) - r.pos;
+    return __any_sync(0xffffffffu, rel < win.hi && rel + V - 1 > -win.w);
   }
   // the unit's elements that belong to the row
   __device__ __forceinline__ void store(const BiasSoftmaxArgs& a, const RowView& r, int u, const uint4& o) const {
@@ -262,17 +297,26 @@ struct Units {
       v[j / 2] = pack2(uint32_t(j - first) < n ? lo : other, uint32_t(j + 1 - first) < n ? hi : other);
     }
   }
-  // x <- scale x + bias; `near`: some lane's unit reaches into the window
-  __device__ __forceinline__ void logits(const RowView& r, const Window<V>& win, uint32_t lut, float left, float right,
-                                         uint64_t scale, int u, bool near, uint64_t* x) const {
+  // x <- scale x + bias
+  __device__ __forceinline__ void logits(const RowView& r, const Window<V>& win, const Lut<V>& lut, uint64_t scale, int u,
+                                         uint64_t* x) const {
     const int rel = key(r, u) - r.pos;
-    if (!near) {
-      const uint64_t bias = both(rel >= win.hi ? right : left);
+    if (!any_near(r, win, u)) {
+      const uint64_t bias = both(rel >= win.hi ? lut.right : lut.left);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) x[j] = fma2(x[j], scale, bias);
+    } else if (lut.columns) {
+      const uint32_t at = lut.shifted(rel);
+#pragma unroll
+      for (int j = 0; j < V / 2; j += 2) {
+        uint64_t b0, b1;
+        asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(b0), "=l"(b1) : "r"(at + 8u * j) : "memory");
+        x[j] = fma2(x[j], scale, b0);
+        x[j + 1] = fma2(x[j + 1], scale, b1);
+      }
     } else {
       // the places from hi on, and those up to -W, hold the constants
-      const Places<V> at(lut, win.place(max(min(rel, win.hi), -win.w - (V - 1))));
+      const Places<V> at(lut.at, win.place(max(min(rel, win.hi), -win.w - (V - 1))));
 #pragma unroll
       for (int j = 0; j < V; j += 2)
         x[j / 2] = fma2(x[j / 2], scale, pack2(ld_shared_f32(at(j)), ld_shared_f32(at(j + 1))));
@@ -291,26 +335,22 @@ __device__ __forceinline__ float lg2_approx(float v) {
   return r;
 }
 
-// v <- exp(v - m); v may be -inf, m is not.  `direct`: |m| is at most 2^100 in
-// every lane.
+// v <- exp(v - m); v may be -inf, m is not.
 template <int N>
-__device__ __forceinline__ void exp_minus(uint64_t* v, float m, bool direct) {
+__device__ __forceinline__ void exp_minus(uint64_t* v, uint64_t minus_m) {
   const uint64_t l = both(kLog2e);
-  if (direct) {
-    const uint64_t nm = both(-m * kLog2e);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = fma2(v[i], l, nm);
-  } else {
-    const uint64_t nm = both(-m);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = mul2(add2(v[i], nm), l);
-  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float lo, hi;
-    unpack2(v[i], lo, hi);
+    unpack2(mul2(add2(v[i], minus_m), l), lo, hi);
     v[i] = pack2(ex2_approx(lo), ex2_approx(hi));
   }
+}
+// The largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // 16-byte words of a thread for one row of one array.
@@ -325,8 +365,8 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   const Team t = team_of(a.shape);
   const Window<V> win(a);
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
-  float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
-  const uint32_t lut_at = shared_address(lut);
+  float* const copies = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
+  float* const window = copies + (a.window_copies ? Lut<V>::words(win) : 0);
   const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
@@ -347,9 +387,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
   copy_async_commit();
   DropRun run{};
   if constexpr (kDrop) run = drop_run(a.drop, a.seed);
-  fill_window(a, win, rows.head, lut);
-  __syncthreads();
-  const float left = lut[0], right = lut[win.word(win.places() - 1)];
+  const Lut<V> lut = fill_window(a, win, rows.head, window, copies);
   const uint64_t scale = both(a.scale);
   const bool two = a.ring_rows == 2;  // a row ahead; else the next one is fetched when this one is read
   // the teams of a warp go on together while one of them has a row
@@ -371,30 +409,28 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
-    const Slots of = units.template slots<U>(r, win, here);
     uint64_t e[U][H];
     float m = kNegInf;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       act_widen2<T>(ld_shared(slot + uint32_t(u) * pitch), e[u]);
-      units.logits(r, win, lut_at, left, right, scale, u, of.near >> u & 1u, e[u]);
-      if (!(of.whole >> u & 1u)) units.mask(r, u, kNegInf, e[u]);
+      units.logits(r, win, lut, scale, u, e[u]);
+      if (!units.all_whole(r, u)) units.mask(r, u, kNegInf, e[u]);
 #pragma unroll
       for (int j = 0; j < H; ++j) {
         float lo, hi;
         unpack2(e[u][j], lo, hi);
-        m = fmaxf(m, fmaxf(lo, hi));
+        m = max3(m, lo, hi);
       }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
       if (uint32_t(d) < t.lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float base = m == kNegInf ? 0.0f : m;  // nothing visible: every 2^x below is 0
-    const bool direct = __all_sync(0xffffffffu, fabsf(base) <= 0x1p100f);
     uint64_t s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      exp_minus<H>(e[u], base, direct);
+      exp_minus<H>(e[u], both(-base));
 #pragma unroll
       for (int j = 0; j < H; j += 2) {
         s2 = add2(s2, e[u][j]);
@@ -423,13 +459,12 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
     // masked keys hold 0 already, unless a NaN in the row makes the factor one
     const bool odd = __any_sync(0xffffffffu, here && !(factor >= 0.0f));
     if (!two && on) fetch(ring);
-    if (!here) continue;
-    if (t.tid == 0 && t.rank == 0) a.lse[this_index] = sum == 0.0f ? kNegInf : __fmaf_rn(lg2_approx(sum), kLn2, top);
+    if (here && t.tid == 0 && t.rank == 0) a.lse[this_index] = sum == 0.0f ? kNegInf : __fmaf_rn(lg2_approx(sum), kLn2, top);
     const uint64_t by = both(kDrop ? factor * run.scale : factor);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (of.seen >> u & 1u) {
+      if (units.any_seen(r, u)) {
         uint64_t* x = e[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], by);
@@ -444,10 +479,10 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_kernel(const __grid
             x[j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
           }
         }
-        if (odd && !(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);
+        if (odd) units.mask(r, u, 0.0f, x);
         o = act_narrow2<T>(x);
       }
-      units.store(a, r, u, o);
+      if (here) units.store(a, r, u, o);
     }
   }
 }
@@ -462,10 +497,10 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   const Window<V> win(a);
   const int teams = int(t.count);
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
-  float* const lut = reinterpret_cast<float*>(dynamic + a.ring_rows * 2 * row_words<T, E>() * blockDim.x);
-  float* const sums = lut + win.words();  // the teams' windows
-  const uint32_t lut_at = shared_address(lut),
-                 mine = shared_address(sums + int(t.index) * win.words());
+  float* const copies = reinterpret_cast<float*>(dynamic + a.ring_rows * 2 * row_words<T, E>() * blockDim.x);
+  float* const window = copies + (a.window_copies ? Lut<V>::words(win) : 0);
+  float* const sums = window + win.words();  // the teams' windows
+  const uint32_t mine = shared_address(sums + int(t.index) * win.words());
   const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
@@ -490,10 +525,8 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   copy_async_commit();
   DropRun run{};
   if constexpr (kDrop) run = drop_run(a.drop, a.seed);
-  fill_window(a, win, rows.head, lut);
   for (int i = int(threadIdx.x); i < teams * win.words(); i += int(blockDim.x)) sums[i] = 0.0f;
-  __syncthreads();
-  const float bias_left = lut[0], bias_right = lut[win.word(win.places() - 1)];
+  const Lut<V> lut = fill_window(a, win, rows.head, window, copies);
   const uint64_t scale = both(a.scale);
   const float drop_scale = kDrop ? run.scale : 1.0f;
   float left = 0.0f, right = 0.0f;  // dl of units wholly at rel <= -W, or at rel >= hi
@@ -515,19 +548,17 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
-    const Slots of = units.template slots<U>(r, win, here);
-    const bool direct = __all_sync(0xffffffffu, fabsf(base) <= 0x1p100f);
     uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
       act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
-      units.logits(r, win, lut_at, bias_left, bias_right, scale, u, of.near >> u & 1u, p[u]);
-      if (!(of.whole >> u & 1u)) {
+      units.logits(r, win, lut, scale, u, p[u]);
+      if (!units.all_whole(r, u)) {
         units.mask(r, u, kNegInf, p[u]);
         units.mask(r, u, 0.0f, d[u]);
       }
-      if (kDrop && (of.seen >> u & 1u)) {
+      if (kDrop && units.any_seen(r, u)) {
         const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
         bool keep[V];
         drop_keep<1, V>(run, i, keep);
@@ -538,7 +569,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
           d[u][j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
         }
       }
-      exp_minus<H>(p[u], base, direct);
+      exp_minus<H>(p[u], both(-base));
 #pragma unroll
       for (int j = 0; j < H; j += 2) {
         s2 = fma2(p[u][j], d[u][j], s2);
@@ -551,26 +582,26 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     // masked keys hold P = 0 already, unless the sum is a NaN or infinite
     const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
     if (!two && on) fetch(ring);
-    if (!here) continue;
     // dl = P (D(dp) - sum): the dropout's scale enters here
     const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (of.seen >> u & 1u) {
+      if (units.any_seen(r, u)) {
         uint64_t* x = p[u];
 #pragma unroll
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
-        if (odd && !(of.whole >> u & 1u)) units.mask(r, u, 0.0f, x);
+        if (odd) units.mask(r, u, 0.0f, x);
         const int rel = units.key(r, u) - r.pos;
-        if (!(of.near >> u & 1u) || rel >= win.hi || rel + V - 1 <= -win.w) {
+        const bool near = units.any_near(r, win, u);
+        if (!near || rel >= win.hi || rel + V - 1 <= -win.w) {
           uint64_t v = x[0];
 #pragma unroll
           for (int j = 1; j < H; ++j) v = add2(v, x[j]);
-          const float f = sum2(v);
+          const float f = here ? sum2(v) : 0.0f;
           left += rel >= win.hi ? 0.0f : f;
           right += rel >= win.hi ? f : 0.0f;
-        } else {
+        } else if (here) {
           const Places<V> at(mine, win.place(rel));
 #pragma unroll
           for (int j = 0; j < H; ++j) {
@@ -584,7 +615,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
         for (int j = 0; j < H; ++j) x[j] = mul2(x[j], scale);
         o = act_narrow2<T>(x);
       }
-      units.store(a, r, u, o);
+      if (here) units.store(a, r, u, o);
     }
   }
   // fold the windows by bucket
@@ -668,7 +699,6 @@ constexpr uint32_t kSharedBytes = 216 * 1024;  // dynamic shared memory of a CTA
 }  // namespace
 
 TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, int sms) {
-  (void)grad;
   const uint64_t v = type == kF32 ? 4 : 8;
   // a row that starts inside a unit spreads over one more
   const uint64_t span = keys % v ? keys + v - 1 : keys;
@@ -680,7 +710,7 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   uint64_t least = UINT64_MAX;
   if (rows >= uint64_t(sms) * 8 && span <= 32 * 40) {
     for (int e : {40, 32, 16}) {
-      uint64_t lanes = 4;
+      uint64_t lanes = grad ? 8 : 4;  // each team of a gradient has a window of its own
       while (span > lanes * uint64_t(e)) lanes *= 2;
       if (lanes <= 32 && lanes * uint64_t(e + 8) < least) {
         least = lanes * uint64_t(e + 8);
@@ -713,9 +743,11 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
 void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad) {
   const uint32_t window = uint32_t(a->type == kF32 ? Window<4>(*a).words() : Window<8>(*a).words()) * 4;
   const uint32_t row = (grad ? 2u : 1u) * uint32_t(a->shape.elems) * (a->type == kF32 ? 4u : 2u);  // bytes of a thread
+  const uint32_t copies = uint32_t(a->type == kF32 ? Lut<4>::words(Window<4>(*a)) : Lut<8>::words(Window<8>(*a))) * 4;
   a->ring_rows = 2;
+  a->window_copies = 0;
   auto total = [&] {
-    return a->ring_rows * row * uint32_t(a->shape.threads) +
+    return a->ring_rows * row * uint32_t(a->shape.threads) + a->window_copies * copies +
            (1 + (grad ? uint32_t(team_count(a->shape)) : 0u)) * window;
   };
   // wide windows leave room for fewer teams, the longest f32 rows for one row at a time
@@ -725,6 +757,8 @@ void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad) {
     else break;
   }
   if (total() > kSharedBytes) a->ring_rows = 1;
+  // the window's copies where a warp's rows are many and they take little
+  a->window_copies = a->shape.warp_teams && copies <= 12 * 1024 && total() + copies <= kSharedBytes ? 1 : 0;
   a->shared_bytes = total();
 }
 

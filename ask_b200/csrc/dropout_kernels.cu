@@ -25,7 +25,7 @@ namespace {
 template <int T, bool kRes>
 constexpr int units_in_flight() { return act_vec<T>() == 8 && !kRes ? 4 : 2; }
 template <int T, bool kRes>
-constexpr int ctas_per_sm() { return act_vec<T>() == 8 ? (kRes ? 3 : 1) : 4; }
+constexpr int ctas_per_sm() { return act_vec<T>() == 8 ? (kRes ? 3 : 2) : 4; }
 
 template <int T>
 __device__ __forceinline__ void load_elems(const void* p, uint64_t i, int n, float* v) {

@@ -288,7 +288,7 @@ struct BiasSoftmaxArgs {
   int thresholds[kBiasMaxThresholds];  // not falling; the bucket of a distance n is the number of them <= n
   DropSite drop;
   TeamShape shape;
-  uint32_t ring_rows, shared_bytes;  // rows in flight (1 or 2), dynamic shared memory of a CTA
+  uint32_t ring_rows, window_copies, shared_bytes;  // rows in flight (1 or 2); the window's copies (0 or 1); of a CTA
 };
 TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, int sms);
 // Threads of a CTA as the windows in shared memory allow, and those bytes.
