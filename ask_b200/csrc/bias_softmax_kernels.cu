@@ -682,8 +682,10 @@ const void* kernel_of_type(const BiasSoftmaxArgs& a, bool grad) {
   const bool even = a.aligned && a.keys % uint32_t(act_vec<T>()) == 0;
   return a.shape.elems == 8    ? kernel_of_fit<T, 8, kDrop>(grad, even)
          : a.shape.elems == 16 ? kernel_of_fit<T, 16, kDrop>(grad, even)
+         : a.shape.elems == 24 ? kernel_of_fit<T, 24, kDrop>(grad, even)
          : a.shape.elems == 32 ? kernel_of_fit<T, 32, kDrop>(grad, even)
-                               : kernel_of_fit<T, 40, kDrop>(grad, even);
+         : even                ? (const void*)bias_softmax_kernel<T, 40, kDrop, true>
+                               : (const void*)bias_softmax_kernel<T, 40, kDrop, false>;
 }
 template <bool kDrop>
 const void* kernel_of(const BiasSoftmaxArgs& a, bool grad) {
@@ -709,7 +711,8 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
   // a warp's 1024), fewer leave a row's work to more threads.
   uint64_t least = UINT64_MAX;
   if (rows >= uint64_t(sms) * 8 && span <= 32 * 40) {
-    for (int e : {40, 32, 16}) {
+    for (int e : {40, 32, 24, 16}) {
+      if (grad && e == 40) continue;  // two rows of 40 elements a thread spill
       uint64_t lanes = grad ? 8 : 4;  // each team of a gradient has a window of its own
       while (span > lanes * uint64_t(e)) lanes *= 2;
       if (lanes <= 32 && lanes * uint64_t(e + 8) < least) {
@@ -718,10 +721,11 @@ TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, 
         s.warp_teams = int(lanes);
       }
     }
-    return s;
+    if (s.warp_teams) return s;
   }
   // few rows take more threads for each
-  for (int e : {40, 32, 16, 8}) {
+  for (int e : {40, 32, 24, 16, 8}) {
+    if (grad && e == 40) continue;
     const uint64_t threads = ((span + uint64_t(e) - 1) / uint64_t(e) + 31) / 32 * 32;
     if (threads > uint64_t(kTeamThreads)) continue;
     const uint64_t cost = rows < uint64_t(sms) * 2 ? uint64_t(e) : threads * uint64_t(e + 8);
