@@ -87,20 +87,30 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
       fac.write(f);
     }
   }
+  // a row's statistics, loaded one row ahead
+  struct {
+    float mean_h, rstd_h, mean_y, rstd_y;
+  } stats;
+  auto load_stats = [&](uint32_t turn, uint64_t r) {
+    stats = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (turn >= mine) return;
+    if (pre) {
+      if (kFull && a.layer) stats.mean_h = __ldg(a.stats_pre_in + 2 * r);
+      stats.rstd_h = __ldg(a.stats_pre_in + (kFull && a.layer ? 2 * r + 1 : r));
+    }
+    if (post) {
+      if (kFull && a.layer) stats.mean_y = __ldg(a.stats_post_in + 2 * r);
+      stats.rstd_y = __ldg(a.stats_post_in + (kFull && a.layer ? 2 * r + 1 : r));
+    }
+  };
+  load_stats(0, row);
   uint64_t acc_t[P] = {}, acc_p[P] = {}, acc_s[kFull ? P : 1] = {}, acc_q[kFull ? P : 1] = {};
   uint32_t slot = ring, free_slot = ring + (S - 1) * stage_bytes;
   for (uint32_t turn = 0; turn < turns; ++turn, row += t.count, off += advance) {
     const int parity = int(turn & 1u);
     const bool on = turn < mine;  // a row that is not there counts as zeros
-    float mean_h = 0.0f, rstd_h = 0.0f, mean_y = 0.0f, rstd_y = 0.0f;
-    if (pre && on) {
-      if (kFull && a.layer) mean_h = __ldg(a.stats_pre_in + 2 * row);
-      rstd_h = __ldg(a.stats_pre_in + (kFull && a.layer ? 2 * row + 1 : row));
-    }
-    if (post && on) {
-      if (kFull && a.layer) mean_y = __ldg(a.stats_post_in + 2 * row);
-      rstd_y = __ldg(a.stats_post_in + (kFull && a.layer ? 2 * row + 1 : row));
-    }
+    const float mean_h = stats.mean_h, rstd_h = stats.rstd_h, mean_y = stats.mean_y, rstd_y = stats.rstd_y;
+    load_stats(turn + 1, row + t.count);
     fetch(turn + S - 1, off + (S - 1) * advance, free_slot);
     copy_async_wait<S - 1>();
     uint64_t g[P];
