@@ -219,7 +219,7 @@ struct TeamShape {
   int elems;       // row elements a thread holds
 };
 
-// Block norms (norm_kernels.cu).  Forward: h = alpha x + D(gate * N_post(y)),
+// Block norms (norm_rows.cuh).  Forward: h = alpha x + D(gate * N_post(y)),
 // u = N_pre(h); gradient: see the kernel.  x, y, h, u and the gradients to
 // them are [rows, cols] of `type`; weights, biases [cols] and gate
 // [groups, cols] of `ptype`; statistics [rows, 1 or 2] and the gradients to
@@ -254,14 +254,15 @@ struct NormSums {
   int count() const { return int(t) + int(s) + int(p) + int(q); }
 };
 NormSums norm_sums(const NormArgs& a);
-cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm);
-cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm);
+// Resident CTAs an SM, and the dynamic shared memory of one.
+cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm, unsigned* shared_bytes);
+cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm, unsigned* shared_bytes);
 cudaError_t norm_launch(const NormArgs& a, NormFit fit, int grid, cudaStream_t stream);
 cudaError_t norm_grad_launch(const NormArgs& a, NormFit fit, cudaStream_t stream);
 // Rows a CTA works on at once.
 inline int team_count(const TeamShape& s) { return s.threads / (s.warp_teams ? s.warp_teams : s.team_threads); }
 
-// Softmax over biased scores (bias_softmax_kernels.cu).  s, p, dp, ds are
+// Softmax over biased scores (bias_softmax.cuh).  s, p, dp, ds are
 // [batch, heads, queries, keys] of `type`, table [buckets, heads] of
 // `table_type`, lengths and offsets i32 [batch] (null: all keys, 0), lse
 // [batch, heads, queries] f32.
@@ -293,8 +294,10 @@ struct BiasSoftmaxArgs {
 TeamShape bias_softmax_shape(uint64_t keys, uint64_t rows, int type, bool grad, int sms);
 // Threads of a CTA as the windows in shared memory allow, and those bytes.
 void bias_softmax_shared(BiasSoftmaxArgs* a, bool grad);
-cudaError_t bias_softmax_occupancy(const BiasSoftmaxArgs& a, bool grad, int* blocks_per_sm);
-cudaError_t bias_softmax_launch(const BiasSoftmaxArgs& a, bool grad, cudaStream_t stream);
+cudaError_t bias_softmax_occupancy(const BiasSoftmaxArgs& a, int* blocks_per_sm);
+cudaError_t bias_softmax_grad_occupancy(const BiasSoftmaxArgs& a, int* blocks_per_sm);
+cudaError_t bias_softmax_launch(const BiasSoftmaxArgs& a, cudaStream_t stream);
+cudaError_t bias_softmax_grad_launch(const BiasSoftmaxArgs& a, cudaStream_t stream);
 
 cudaError_t gen_launch(int kind, uint64_t seed, uint32_t stream_id, uint64_t offset, uint64_t count, double p0,
                        double p1, const double* zipf_cdf, uint64_t zipf_n, void* dst, cudaStream_t stream);

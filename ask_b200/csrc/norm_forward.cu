@@ -177,8 +177,9 @@ TeamShape norm_shape(uint64_t cols, int type, bool grad) {
   return s;
 }
 
-cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
+cudaError_t norm_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm, unsigned* shared_bytes) {
   const Chosen c = choose<Pick>(a, fit);
+  *shared_bytes = c.shared_bytes;
   const cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
   if (e != cudaSuccess) return e;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);

@@ -348,8 +348,9 @@ NormSums norm_sums(const NormArgs& a) {
   return NormSums{a.branch && (a.post || a.gated), a.post && a.bias, bool(a.pre), a.pre && a.bias};
 }
 
-cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm) {
+cudaError_t norm_grad_occupancy(const NormArgs& a, NormFit fit, int* blocks_per_sm, unsigned* shared_bytes) {
   const Chosen c = choose<Pick>(a, fit);
+  *shared_bytes = c.shared_bytes;
   const cudaError_t e = prepare_rows(c.kernel, c.shared_bytes);
   if (e != cudaSuccess) return e;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks_per_sm, c.kernel, a.shape.threads, c.shared_bytes);

@@ -1022,7 +1022,8 @@ void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
   int occ = 2;
   if (pl.device >= 0) {
     const NormFit fit = norm_fit(a, 0);
-    check_cuda(grad ? norm_grad_occupancy(a, fit, &occ) : norm_occupancy(a, fit, &occ), "occupancy");
+    check_cuda(grad ? norm_grad_occupancy(a, fit, &occ, &pl.shared) : norm_occupancy(a, fit, &occ, &pl.shared),
+               "occupancy");
   }
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
@@ -1109,7 +1110,9 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
   bias_softmax_shared(&a, grad);
   pl.block = a.shape.threads;
   int occ = 2;
-  if (pl.device >= 0) check_cuda(bias_softmax_occupancy(a, grad, &occ), "occupancy");
+  pl.shared = a.shared_bytes;
+  if (pl.device >= 0)
+    check_cuda(grad ? bias_softmax_grad_occupancy(a, &occ) : bias_softmax_occupancy(a, &occ), "occupancy");
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
   const uint64_t teams = uint64_t(team_count(a.shape));
@@ -1173,7 +1176,7 @@ std::string describe(const ask_b200_plan& pl) {
     << ",\"target\":{\"backend\":\"cuda\",\"arch\":100},\"launch\":{\"grid\":[" << pl.grid << "," << pl.col_chunks << ",1],\"block\":["
     << (pl.sm_step ? pl.block : pl.family == FAM_ELEMENTWISE ? kEwThreads : pl.family == FAM_REDUCE ? kRedThreads :
         row_family(pl.family) ? pl.block : 256)
-    << ",1,1],\"shared_bytes\":0},\"kernels_per_launch\":" << pl.launches << ",\"scratch_bytes\":" << pl.scratch;
+    << ",1,1],\"shared_bytes\":" << pl.shared << "},\"kernels_per_launch\":" << pl.launches << ",\"scratch_bytes\":" << pl.scratch;
   if (pl.family == FAM_REDUCE) {
     const char* strat[] = {"warp_row", "column", "split"};
     o << ",\"strategy\":\"" << (pl.sm_step ? "row_cta" : pl.views ? "view" : strat[pl.strategy]) << "\",\"shardable\":" << (pl.shardable ? "true" : "false")
@@ -1199,7 +1202,7 @@ std::string describe(const ask_b200_plan& pl) {
                     : pl.family == FAM_REDUCE ? kRedThreads
                     : row_family(pl.family) ? pl.block : 256;
   o << "],\"invocation\":{\"version\":2,\"kind\":\"ask-b200-recipe\",\"grid\":[" << pl.grid
-    << ",1,1],\"block\":[" << block << ",1,1],\"shared_bytes\":0,\"arguments\":[";
+    << ",1,1],\"block\":[" << block << ",1,1],\"shared_bytes\":" << pl.shared << ",\"arguments\":[";
   for (size_t k = 0; k < pl.inputs.size() + pl.outputs.size(); ++k)
     o << (k ? "," : "") << "\"" << (k < pl.inputs.size() ? "input:" : "output:")
       << (k < pl.inputs.size() ? k : k - pl.inputs.size()) << "\"";
@@ -1458,7 +1461,7 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
       if (pl.scratch && !scratch) fail(ASK_B200_E_INVALID, "this plan needs scratch memory");
       if (scratch && !aligned16(scratch)) fail(ASK_B200_E_INVALID, "scratch must be 16-byte aligned");
       a.partial = reinterpret_cast<float*>(scratch);
-      check_cuda(bias_softmax_launch(a, grad, st), "bias_softmax launch");
+      check_cuda(grad ? bias_softmax_grad_launch(a, st) : bias_softmax_launch(a, st), "bias_softmax launch");
       break;
     }
     default:

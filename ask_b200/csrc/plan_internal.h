@@ -45,7 +45,8 @@ struct ask_b200_plan {
   askb::ViewSet vs{};
   bool shardable = false;
   std::string kernel;
-  int block = 256;  // threads per CTA where the family fixes it (softmax)
+  int block = 256;  // threads per CTA where the family fixes it (softmax and the block operators)
+  unsigned shared = 0;  // dynamic shared memory of a CTA (the block operators on a device)
   int col_chunks = 1;  // RS_COLUMN: chunks of the extent over grid.y (1 = the one-pass column kernel)
   int blocks_per_sm = 0;  // recipe cap on resident CTAs per SM of a persistent grid (0 = occupancy)
   int sm_step = 0;   // reduce matched to a softmax step run by the softmax row kernel (SoftmaxMode), else 0

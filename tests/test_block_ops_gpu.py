@@ -202,6 +202,14 @@ def test_block_norm_widths(device, dtype, params, cols):
     run_norm(dtype, params, 6, cols, SWITCHES[2])
 
 
+@pytest.mark.parametrize("dtype,params", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("cols", [3, 10, 62, 130, 514, 515, 1030, 1031, 8194, 8195, 16386])
+@pytest.mark.parametrize("switch", [SWITCHES[1], SWITCHES[2], SWITCHES[7]])
+def test_block_norm_rows_off_the_units(device, dtype, params, cols, switch):
+    """Rows of whole words, of odd numbers of 16-bit elements, and f32 rows, none of whole 16-byte units."""
+    run_norm(dtype, params, 12, cols, switch)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 601, 5000])
 @pytest.mark.parametrize("cols", [96, 1000])
 def test_block_norm_row_counts(device, rows, cols):
@@ -307,6 +315,14 @@ def test_bias_softmax_many_rows(device, dtype, shape, both, causal, lens, p):
     """Enough rows for a warp each; lengths of zero and one among them."""
     lengths = [[0, 1, shape[3], shape[3] // 2, 3][b % 5] for b in range(shape[0])] if lens else None
     run_softmax(dtype, shape, TH if both else TH1, both, 0.25, causal, lengths, None, p)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("keys", [1, 5, 33, 64, 65, 96, 100, 128, 200, 257, 384, 520, 768, 1000, 1021, 1024, 1030, 1101, 1280])
+def test_bias_softmax_rows_of_a_warp_or_less(device, dtype, keys):
+    """1200 rows: every share of a warp and number of elements a thread, odd keys and offsets among them."""
+    run_softmax(dtype, (4, 2, 150, keys), TH, True, 0.5, keys % 3 == 0, [keys, keys // 2 + 1, 0, 1], [0, 7, -3, 150],
+                p=0.25 if keys % 2 else 0.0)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
@@ -464,6 +480,28 @@ def test_graph_replay_draws_new_masks(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y.cpu(), dropout_exact(np.ones(n), None, 0.5, 1, step * 2500, 0, "f32"))
+
+
+def test_first_launch_inside_a_capture(device):
+    """A plan whose ports turn out unaligned takes another kernel than the one it was made for: also under capture."""
+    rows, cols = 40, 256
+    rng = np.random.default_rng(6)
+    for dtype, skew in (("f32", 1), ("bf16", 1), ("bf16", 2)):
+        xs = dev(rounded(rng, (rows, cols), dtype), dtype, skew)
+        w = dev(np.ones(cols), "f32")
+        u, s = torch.empty(rows * cols + 8, dtype=TORCH[dtype], device="cuda")[skew:skew + rows * cols], torch.empty(rows, device="cuda")
+        plan = ask_b200.Plan(R.block_norm(dtype, rows, cols, branch=False, eps=1e-5), device=0)
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            plan.launch([xs, w], [u, s], None, stream)
+        graph.replay()
+        torch.cuda.synchronize()
+        v = host(xs, (rows, cols))
+        _, rstd = ref.stats(v, False, 1e-5)
+        want = v * rstd[:, None]
+        close(host(u, (rows, cols)), want, ref.stored(want, np.abs(want), dtype), "u")
 
 
 def test_missing_scratch_and_ports_are_errors(device):
