@@ -269,20 +269,24 @@ struct Units {
       st_stream_v4(to, o);
       return;
     }
+    // a cut unit: elements [first, end), by words and the halves at either end
     const uint32_t w[4] = {o.x, o.y, o.z, o.w};
     const int first = max(-k0, 0), end = min(keys - k0, V);
+    if constexpr (B == 4) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {  // by words, and by halves of them
-      if constexpr (B == 4) {
+      for (int k = 0; k < 4; ++k)
         if (k >= first && k < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
-      } else {
-        const bool lo = 2 * k >= first && 2 * k < end, hi = 2 * k + 1 >= first && 2 * k + 1 < end;
-        if (lo && hi && a.aligned) reinterpret_cast<uint32_t*>(to)[k] = w[k];
-        else {
-          if (lo) reinterpret_cast<uint16_t*>(to)[2 * k] = uint16_t(w[k]);
-          if (hi) reinterpret_cast<uint16_t*>(to)[2 * k + 1] = uint16_t(w[k] >> 16);
-        }
-      }
+    } else if (a.aligned) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (2 * k >= first && 2 * k + 1 < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+      const auto word = [&](int e) { return e < 4 ? (e < 2 ? w[0] : w[1]) : (e < 6 ? w[2] : w[3]); };
+      if (first & 1) reinterpret_cast<uint16_t*>(to)[first] = uint16_t(word(first) >> 16);
+      if ((end & 1) && end > first) reinterpret_cast<uint16_t*>(to)[end - 1] = uint16_t(word(end - 1));
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j >= first && j < end) reinterpret_cast<uint16_t*>(to)[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));
     }
   }
   // v <- v where the key is visible, else `other`
