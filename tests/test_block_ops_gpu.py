@@ -580,3 +580,46 @@ def test_offsets_past_32_bits(device):
     assert bool((last[1000:] == 0).all()) and abs(float(last[999]) * 1000 - 1) <= 2.0 ** -10
     assert abs(float(lse[-1]) - math.log(1000)) <= 1e-5 and float(lse[0]) == -math.inf
     assert bool((p[:shape[3]] == 0).all())
+
+
+# ---- the operators together -------------------------------------------------------------------------
+def test_encoder_block_example(device):
+    """examples/encoder_block.py in f32 against torch's own differentiation of the same block in 64 bits, with the
+    masks of the published generator."""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("encoder_block", os.path.join(
+        os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "encoder_block.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    b, n, d, h, p = 3, 20, 48, 4, 0.2
+    block = mod.EncoderBlock(b, n, d, h, dtype="f32", dropout=p)
+    torch.backends.cuda.matmul.allow_tf32 = False
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    embedding = torch.randn(b * n, d, device="cuda", generator=gen)
+    dz = torch.randn(b * n, d, device="cuda", generator=gen)
+    lens = [n, 13, 1]
+    z = block.forward(embedding, dev(np.array(lens), "i32"), dev(np.array([77, 5]), "i64"))
+    grads = block.backward(dz)
+
+    mask = lambda shape, stream: torch.from_numpy(ref.drop_factor((p, 77, 5, stream), shape))  # noqa: E731
+    leaf = lambda t: t.detach().double().cpu().requires_grad_()  # noqa: E731
+    e = leaf(embedding)
+    w = {k: leaf(v) for k, v in block.weights.items()}
+    table, w1, w2, w3, gate = (leaf(t) for t in (block.table, block.w_first, block.w_post, block.w_pre, block.gate))
+    rms = lambda t, weight: t * (t.square().mean(1, keepdim=True) + 1e-6).rsqrt() * weight  # noqa: E731
+    x = e * mask((b * n, d), 0)
+    u = rms(x, w1)
+    q, k, v = ((u @ w[c]).view(b, n, h, d // h).transpose(1, 2) for c in "qkv")
+    seen, _, ids = ref.masks_and_bias((b, h, n, n), block.table.double().cpu().numpy(), TH, True, False, lens, None)
+    logits = q @ k.transpose(2, 3) / math.sqrt(d // h) + table[torch.from_numpy(ids)].permute(0, 3, 1, 2)
+    prob = torch.softmax(logits.masked_fill(~torch.from_numpy(seen), -math.inf), 3) * mask((b, h, n, n), 1)
+    y = (prob @ v).transpose(1, 2).reshape(b * n, d) @ w["o"]
+    out = rms(x + rms(y, w2) * gate * mask((b * n, d), 2), w3)
+    out.backward(dz.double().cpu())
+    want = {"embedding": e, "table": table, "w_first": w1, "w_post": w2, "w_pre": w3, "gate": gate, **w}
+    out = out.detach()
+    assert float((z.double().cpu() - out).abs().max()) <= 1e-4 * float(out.abs().max())
+    for name, t in want.items():
+        got = grads[name].double().cpu().view(t.shape)
+        assert float((got - t.grad).norm()) <= 1e-4 * float(t.grad.norm()), name
