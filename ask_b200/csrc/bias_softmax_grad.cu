@@ -1,4 +1,9 @@
 // Softmax of biased scores, gradient: see bias_softmax.cuh.
+//
+// One pass: P is recomputed from s and lse, so besides s and dp nothing of the
+// forward pass is read.  Each team has a window of its own for the table's
+// gradient; adds of a row go to distinct places, and rows follow each other
+// behind the team's reduction, so sums have one order and no atomics.
 #include "bias_softmax.cuh"
 
 namespace askb {

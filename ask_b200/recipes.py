@@ -16,6 +16,21 @@ The five benchmark configurations are provided as step recipes:
 * :func:`cfg4_gather_step`, :func:`cfg4_scatter_step` -- embedding gather and
   scatter_add (with the runtime pre_copy of the base into the output).
 * :func:`cfg5a_step`, :func:`cfg5b_step` -- the sharded plan's two parts.
+
+Five families beyond ASK's owned steps are the row work of a transformer block
+between its matrix products, for training and for single tokens:
+
+* :func:`dropout` -- dropout (+ residual) with the mask drawn from a counter.
+* :func:`block_norm`, :func:`block_norm_grad` -- a branch's output normed, gated,
+  dropped and added to the residual stream, and the norm of the sum.
+* :func:`bias_softmax`, :func:`bias_softmax_grad` -- masked softmax of scores with
+  a learned relative-position bias (:func:`bucket_thresholds`), and dropout.
+
+Their types are f32, f16 and bf16; sums, statistics and parameter gradients are
+f32.  The seed port is i64[2] {seed, offset} in device memory: element i of a
+tensor uses word i % 4 of Philox4x32-10 at counter (offset + i / 4, stream_id, 1)
+under key seed, so a gradient draws its forward step's mask again, and a
+captured graph draws new ones when the tensor changes.
 """
 from __future__ import annotations
 
@@ -189,7 +204,7 @@ def bias_softmax(dtype: str, batch: int, heads: int, queries: int, keys: int, th
 
     Buckets count the thresholds at or below the distance (``bidirectional``: twice
     len(thresholds) + 1 of them, the second half for keys after the query).  A row
-    without keys gives zeros and lse = -inf.  Single tokens: queries = 1, offsets =
+    without keys, or with -inf in all of them, gives zeros and lse = -inf.  Single tokens: queries = 1, offsets =
     the token's position."""
     return _bias_softmax("bias_softmax", dtype, batch, heads, queries, keys, thresholds, bidirectional, scale, causal,
                          lengths, offsets, dropout, stream_id, table_dtype)
