@@ -114,6 +114,24 @@ __device__ __forceinline__ void store_anywhere(char* p, const uint4& own, int n,
   }
 }
 
+// Elements [first, end) of a 16-byte unit at `to`, by words and the halves at either end.
+template <int T>
+__device__ __forceinline__ void store_cut(char* to, const uint4& own, int first, int end) {
+  const uint32_t w[4] = {own.x, own.y, own.z, own.w};
+  if constexpr (T == kF32) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k >= first && k < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (2 * k >= first && 2 * k + 1 < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+    const auto word = [&](int e) { return e < 4 ? (e < 2 ? w[0] : w[1]) : (e < 6 ? w[2] : w[3]); };
+    if ((first & 1) && end > first) reinterpret_cast<uint16_t*>(to)[first] = uint16_t(word(first) >> 16);
+    if ((end & 1) && end > first) reinterpret_cast<uint16_t*>(to)[end - 1] = uint16_t(word(end - 1));
+  }
+}
+
 // What a thread holds of a row before it is widened: 16 bytes.
 template <int T, int V>
 struct ActRaw {
@@ -148,6 +166,9 @@ __device__ __forceinline__ uint32_t ld_shared_word(uint32_t at) {
 }
 __device__ __forceinline__ void st_shared_word(uint32_t at, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared_half(uint32_t at, uint16_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
 }
 __device__ __forceinline__ void copy_word_to_shared(uint32_t at, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");

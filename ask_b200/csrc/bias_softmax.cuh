@@ -37,7 +37,7 @@
 // among them, and with dropout the generator's 21 clocks more.  bf16 [8, 16, 1024, 1024]: 95 us full
 // and without dropout (5.6 TB/s), 177 us with dropout and ragged lengths;
 // gradient 148 and 233 us.  Rows that are not whole units add masks, cut
-// stores and a unit more a row (1021 keys: 283 us).
+// stores and a unit more a row (1021 keys: 262 us).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -276,21 +276,11 @@ struct Units {
       st_stream_v4(to, o);
       return;
     }
-    // a cut unit: elements [first, end), by words and the halves at either end
-    const uint32_t w[4] = {o.x, o.y, o.z, o.w};
     const int first = max(-k0, 0), end = min(keys - k0, V);
-    if constexpr (B == 4) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k >= first && k < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
-    } else if (a.aligned) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (2 * k >= first && 2 * k + 1 < end) reinterpret_cast<uint32_t*>(to)[k] = w[k];
-      const auto word = [&](int e) { return e < 4 ? (e < 2 ? w[0] : w[1]) : (e < 6 ? w[2] : w[3]); };
-      if (first & 1) reinterpret_cast<uint16_t*>(to)[first] = uint16_t(word(first) >> 16);
-      if ((end & 1) && end > first) reinterpret_cast<uint16_t*>(to)[end - 1] = uint16_t(word(end - 1));
-    } else {
+    if (B == 4 || a.aligned) {
+      store_cut<T>(to, o, first, end);
+    } else {  // a 16-bit tensor may begin inside a word
+      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (j >= first && j < end) reinterpret_cast<uint16_t*>(to)[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));

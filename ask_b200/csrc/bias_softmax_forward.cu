@@ -7,9 +7,10 @@ namespace {
 
 // kSmall: CTAs of 128 threads at most, five an SM (102 registers): single tokens
 // against 4096 keys took 10.7 us so and 11.6 with what the compiler takes by
-// itself; 40 elements a thread do not fit in them.
+// itself (six: 11.4, and rows of 1024 keys 183 for 177); 40 elements a thread
+// take four (1021 keys: 262 us, and 282 with three).
 template <int T, int E, bool kDrop, bool kEven, bool kSmall>
-__global__ void __launch_bounds__(kSmall ? kWarpTeamThreads : kTeamThreads, kSmall && E <= 32 ? 5 : 1)
+__global__ void __launch_bounds__(kSmall ? kWarpTeamThreads : kTeamThreads, kSmall ? (E <= 32 ? 5 : 4) : 1)
     bias_softmax_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
   constexpr int V = act_vec<T>(), U = E / V, H = V / 2;
   extern __shared__ uint4 dynamic[];

@@ -240,14 +240,19 @@ struct NormArgs {
   float alpha, eps;
   int type, ptype;
   int branch, post, pre, layer, bias, gated;
+  // Rows begin at `classes` different places of a 16-byte unit (a power of two; 1
+  // too where they are not read as cut units).
+  // `spread` neighbouring CTAs (or clusters) share a stretch of rows, so that each
+  // team's rows begin at one of them.
+  uint32_t classes, spread;
   DropSite drop;
   TeamShape shape;
 };
 constexpr int kNormMaxCols = 32768;
-TeamShape norm_shape(uint64_t cols, int type, bool grad);
-// How rows lie in memory: whole 16-byte units, whole 4-byte words, or anywhere
-// (16-bit types: an odd number of columns, or a tensor that starts inside a word).
-enum NormFit { NORM_UNITS = 0, NORM_WORDS = 1, NORM_ANYWHERE = 2 };
+void norm_layout(NormArgs* a, bool grad);  // sets shape and classes
+// How rows are read: as whole 16-byte units; as the units of the aligned tensor,
+// cut at the rows' ends; else f32 by words and 16-bit types from anywhere.
+enum NormFit { NORM_UNITS = 0, NORM_CUT = 1, NORM_WORDS = 2, NORM_ANYWHERE = 3 };
 // Row sums the gradient keeps for each column: of B*yhat, B, du*hhat, du.
 struct NormSums {
   bool t, s, p, q;

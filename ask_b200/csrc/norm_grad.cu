@@ -9,7 +9,8 @@
 // sum over a group's rows thus serves both the gate's gradient and the
 // weight's.  A CTA keeps the sums of its rows' columns in registers, leaves them
 // once in scratch, and a second kernel joins the CTAs' sums in order: results do
-// not depend on the order of execution.  bf16 [32768, 4096] takes 321 us with
+// not depend on the order of execution.  What hhat and yhat hold where there is no
+// column meets du = 0 and c = 0.  bf16 [32768, 4096] takes 319 us with
 // dropout (5.0 TB/s) and 270 without; f16 [4099, 1000] layer norms 28-31 us,
 // mostly the latency of two dependent kernels.
 #include "norm_rows.cuh"
@@ -39,18 +40,24 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
   extern __shared__ uint4 dynamic[];
   __shared__ TeamRecords<N> sh[2];
   const Team t = team_of(a.shape);
-  const Cols col(t, a);
   const uint32_t place = blockIdx.x / t.ctas, group = place / a.chunks, chunk = place % a.chunks;
-  const uint64_t begin = uint64_t(group) * a.rows_per_group + a.rows_per_group * chunk / a.chunks;
-  const uint64_t end = uint64_t(group) * a.rows_per_group + a.rows_per_group * (chunk + 1) / a.chunks;
-  uint64_t row = begin + t.index;
-  const uint32_t mine = row < end ? uint32_t((end - row + t.count - 1) / t.count) : 0;
+  const uint32_t stretch = chunk / a.spread, stretches = a.chunks / a.spread, stride = t.count * a.spread;
+  const uint64_t begin = uint64_t(group) * a.rows_per_group + a.rows_per_group * stretch / stretches;
+  const uint64_t end = uint64_t(group) * a.rows_per_group + a.rows_per_group * (stretch + 1) / stretches;
+  // the teams of a warp add their column sums, so their rows begin at the same place of a unit
+  const uint32_t warp = threadIdx.x >> 5, of_warp = 32u / t.lanes;
+  const uint32_t order_in = a.shape.warp_teams
+                                ? warp % a.classes + a.classes * (warp / a.classes * of_warp + t.index % of_warp)
+                                : t.index;
+  uint64_t row = begin + chunk % a.spread * t.count + order_in;
+  const Cols col(t, a, row);
+  const uint32_t mine = row < end ? uint32_t((end - row + stride - 1) / stride) : 0;
   const uint32_t turns = __shfl_sync(0xffffffffu, mine, 0);  // of the warp: its first team has the most rows
   const float inv_cols = 1.0f / float(a.cols);
   const uint32_t ring = Cols::ring(dynamic), array = blockDim.x * uint32_t(Cols::kArrayBytes), stage_bytes = 4 * array;
   const uint32_t pitch = blockDim.x * 16, params = shared_address(dynamic) + S * stage_bytes + threadIdx.x * 16;
   const ParamSlot pre_w{params, pitch}, fac{params + E / 4 * pitch, pitch};
-  const uint64_t bytes = a.rows * a.cols * uint64_t(Cols::B), advance = t.count * uint64_t(a.cols) * Cols::B;
+  const uint64_t bytes = a.rows * a.cols * uint64_t(Cols::B), advance = stride * uint64_t(a.cols) * Cols::B;
   pdl_enter();
   team_start(t);
   DropRun run{};
@@ -109,23 +116,24 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
   load_stats(0, row);
   uint64_t acc_t[P] = {}, acc_p[P] = {}, acc_s[kFull ? P : 1] = {}, acc_q[kFull ? P : 1] = {};
   uint32_t slot = ring, free_slot = ring + (S - 1) * stage_bytes;
-  for (uint32_t turn = 0; turn < turns; ++turn, row += t.count, off += advance) {
+  for (uint32_t turn = 0; turn < turns; ++turn, row += stride, off += advance) {
     const int parity = int(turn & 1u);
     const bool on = turn < mine;  // a row that is not there counts as zeros
     const float mean_h = stats.mean_h, rstd_h = stats.rstd_h, mean_y = stats.mean_y, rstd_y = stats.rstd_y;
-    load_stats(turn + 1, row + t.count);
+    load_stats(turn + 1, row + stride);
     fetch(turn + S - 1, off + (S - 1) * advance, free_slot);
     copy_async_wait<S - 1>();
+    col.trim(slot, 4, array);
     uint64_t g[P];
     if (pre) {
       uint64_t du[P], hh[P];
-      col.read(slot + array, a.du, off, du);
-      col.read(slot + 2 * array, a.h_in, off, hh);
+      col.template read<false>(slot + array, a.du, off, du);
+      col.template read<false>(slot + 2 * array, a.h_in, off, hh);
       if (!on) {
 #pragma unroll
         for (int k = 0; k < P; ++k) du[k] = hh[k] = 0;
       }
-      if (kFull && a.layer) col.center(mean_h, hh);
+      if (kFull && a.layer) col.template center<false>(mean_h, hh);
       const uint64_t r2 = both(rstd_h);
 #pragma unroll
       for (int k = 0; k < P; ++k) {
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
       team_sum<N, true>(t, sh[0], parity, s);
       const uint64_t k2 = both(-s[0] * inv_cols);
       if (branch) {
-        col.read(slot, a.dh, off, g);
+        col.template read<false>(slot, a.dh, off, g);
       } else {
 #pragma unroll
         for (int k = 0; k < P; ++k) g[k] = 0;
@@ -152,7 +160,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
         g[k] = fma2(r2, v, g[k]);
       }
     } else {
-      col.read(slot, a.dh, off, g);
+      col.template read<false>(slot, a.dh, off, g);
     }
     if (!on) {
 #pragma unroll
@@ -169,13 +177,13 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
       if constexpr (kDrop) col.drop(run, off, g);
       if (need_y) {
         uint64_t yy[P];
-        col.read(slot + 3 * array, a.y, off, yy);
+        col.template read<false>(slot + 3 * array, a.y, off, yy);
         if (!on) {
 #pragma unroll
           for (int k = 0; k < P; ++k) yy[k] = 0;
         }
         if (post) {
-          if (kFull && a.layer) col.center(mean_y, yy);
+          if (kFull && a.layer) col.template center<false>(mean_y, yy);
           scale_all(yy, rstd_y);
         }
 #pragma unroll
@@ -245,7 +253,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (j < col.count(q)) to[col.at(q) + j] = v[q * V + j];
+          if (col.has(q, j)) to[col.at(q) + j] = v[q * V + j];
       }
     }
   };

@@ -17,16 +17,14 @@
 // holds what is on its way.  Its parameters lie beside them in shared memory for
 // all of its rows.  Arithmetic runs on f32 pairs.  (Rows prefetched into
 // registers and parameters reloaded for each row took 446 us where this takes
-// 243, the gradient 831 where it takes 321.)
+// 231, the gradient 831 where it takes 319.)
 //
-// Bound: HBM, four tensors forward and six for the gradient, up to 4096
-// columns without dropout (bf16 [32768, 4096]: 180 us = 6.0 TB/s, gradient 270 us =
-// 6.0 TB/s); with dropout the generator's products share the issue slots (243 and
-// 321 us).  Rows of 8192 columns have one team an SM, whose loads wait
-// while it reduces (156 us for half the elements, gradient 221), and those over a
-// cluster wait for its barriers (16384: 236 and 282).  Rows off whole units
-// spend three to four times the address arithmetic (NORM_ANYWHERE: bf16 [8191, 4095]
-// 136 us; a quarter of [32768, 4096] is 61).
+// Bound: HBM, four tensors forward and six for the gradient, up to 6400
+// columns without dropout (bf16 [32768, 4096]: 188 us = 5.7 TB/s, gradient 270 us =
+// 6.0 TB/s); with dropout the generator's products share the issue slots (231 and
+// 319 us).  Wider rows have one team an SM, whose loads wait while it reduces
+// (8192 columns: 161 us for half the elements, gradient 219), and those over a
+// cluster wait for its barriers (16384: 238 and 284).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -51,27 +49,45 @@ enum NormForm { FORM_ANY = 0, FORM_BOTH = 1 /* branch, post and pre norm */, FOR
                 FORM_NORM = 3 /* pre norm alone */ };
 
 // The team's columns of a row, as the thread holds them: kElems / V units of V
-// elements.  A unit is 16 bytes (NORM_UNITS), a 4-byte word (NORM_WORDS: single
-// f32 columns or pairs of 16-bit ones, lane after lane), or 16 bytes that begin
-// anywhere (NORM_ANYWHERE: it spans two aligned words, from which it is shifted
-// out, and stores are put together across lanes).  A row is named by the byte
-// offset of this thread's first column.
+// elements.  A unit is 16 bytes of the row (NORM_UNITS); an aligned unit of the
+// tensor, of which the row's first and last may hold neighbours' elements that
+// count as zeros and are not written (NORM_CUT: all rows of a team begin at the
+// same place of a unit, so its columns and parameters stay as they are); an f32
+// (NORM_WORDS, lane after lane); or 16 bytes that begin anywhere (NORM_ANYWHERE,
+// 16-bit types: it spans two aligned words, from which it is shifted out, and
+// stores are put together across lanes).  A row is named by the byte offset of
+// this thread's first column.
 template <int T, int F>
 struct Columns {
   static constexpr int E = kElems, P = kPairs, B = dtype_bytes(T);
   static constexpr int kUnitBytes = F == NORM_WORDS ? 4 : 16, V = kUnitBytes / B, Q = E / V;
   static constexpr int kCopies = F == NORM_ANYWHERE ? 2 : 1;     // words of a unit in the ring
   static constexpr int kArrayBytes = Q * kCopies * kUnitBytes;   // of a thread, for one row of one array
-  uint32_t first, step;  // column of unit q: first + q * step
-  uint32_t cols, pitch;  // pitch: between a thread's words in shared memory
-  __device__ __forceinline__ Columns(const Team& t, const NormArgs& a)
-      : first((t.rank * uint32_t(Q) * t.threads + t.tid) * uint32_t(V)), step(t.threads * uint32_t(V)), cols(a.cols),
-        pitch(blockDim.x * uint32_t(kUnitBytes)) {}
-  __device__ __forceinline__ uint32_t at(int q) const { return first + uint32_t(q) * step; }
+  int first, step;  // column of unit q: first + q * step
+  int cols;
+  uint32_t pitch;  // between a thread's words in shared memory
+  uint32_t cuts;   // bit q: the warp's units q are not all whole (NORM_CUT)
+  __device__ __forceinline__ Columns(const Team& t, const NormArgs& a, uint64_t row)
+      : first(int((t.rank * uint32_t(Q) * t.threads + t.tid) * uint32_t(V))), step(int(t.threads) * V), cols(int(a.cols)),
+        pitch(blockDim.x * uint32_t(kUnitBytes)), cuts(0) {
+    if constexpr (F == NORM_CUT) {
+      first -= int(uint32_t(row * a.cols) & uint32_t(V - 1));
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        if (__any_sync(0xffffffffu, in(q) && count(q) < V)) cuts |= 1u << q;
+    }
+  }
+  __device__ __forceinline__ int at(int q) const { return first + q * step; }
   __device__ __forceinline__ bool in(int q) const { return at(q) < cols; }
-  __device__ __forceinline__ int count(int q) const { return in(q) ? int(min(cols - at(q), uint32_t(V))) : 0; }
-  __device__ __forceinline__ uint64_t offset(uint64_t row) const { return (row * cols + first) * uint64_t(B); }
-  __device__ __forceinline__ uint64_t unit(uint64_t off, int q) const { return off + uint32_t(q) * step * uint32_t(B); }
+  // unit q's elements [low(q), high(q)) are columns of the row
+  __device__ __forceinline__ int low(int q) const { return F == NORM_CUT ? max(-at(q), 0) : 0; }
+  __device__ __forceinline__ int high(int q) const { return max(min(cols - at(q), V), 0); }
+  __device__ __forceinline__ int count(int q) const { return high(q) - (in(q) ? low(q) : 0); }
+  __device__ __forceinline__ bool has(int q, int j) const { return j >= low(q) && j < high(q); }
+  __device__ __forceinline__ uint64_t offset(uint64_t row) const {
+    return (row * uint32_t(cols) + uint64_t(int64_t(first))) * uint64_t(B);
+  }
+  __device__ __forceinline__ uint64_t unit(uint64_t off, int q) const { return off + uint32_t(q * step * B); }
   __device__ __forceinline__ static uint32_t ring(const void* shared) {
     return shared_address(shared) + threadIdx.x * uint32_t(kUnitBytes);
   }
@@ -86,6 +102,9 @@ struct Columns {
       const uint64_t o = unit(off, q);
       if constexpr (F == NORM_UNITS) {
         copy_to_shared(slot + uint32_t(q) * pitch, begin + o);
+      } else if constexpr (F == NORM_CUT) {
+        if (o + 16 <= bytes) copy_to_shared(slot + uint32_t(q) * pitch, begin + o);
+        else st_shared(slot + uint32_t(q) * pitch, load_part<T>(begin + o, begin, begin + bytes));
       } else if constexpr (F == NORM_WORDS) {
         copy_word_to_shared(slot + uint32_t(q) * pitch, begin + o);
       } else {
@@ -105,27 +124,53 @@ struct Columns {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       if (in(q)) continue;
-      if constexpr (F == NORM_UNITS) st_shared(slot + uint32_t(q) * pitch, make_uint4(0u, 0u, 0u, 0u));
+      if constexpr (F == NORM_UNITS || F == NORM_CUT) st_shared(slot + uint32_t(q) * pitch, make_uint4(0u, 0u, 0u, 0u));
       if constexpr (F == NORM_WORDS) st_shared_word(slot + uint32_t(q) * pitch, 0u);
     }
   }
-  __device__ __forceinline__ void read(uint32_t slot, const void* p, uint64_t off, uint64_t (&v)[P]) const {
-    if constexpr (F == NORM_UNITS) {
+  // Cut units' elements of neighbouring rows count as zeros.  The forward kernel masks
+  // what it reads (kMask); the gradient has no registers for that, and zeroes
+  // them where they lie, in `arrays` arrays of a stage (f32 [33520, 1001]
+  // gradients 216 us masked, 173 so; forward 107 masked, 112 so).
+  __device__ __forceinline__ void trim(uint32_t slot, int arrays, uint32_t array) const {
+    if constexpr (F == NORM_CUT) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) act_widen2<T>(ld_shared(slot + uint32_t(q) * pitch), v + q * V / 2);
-    } else if constexpr (F == NORM_WORDS) {
-      if constexpr (T == kF32) {
+      for (int q = 0; q < Q; ++q) {
+        if (!(cuts & 1u << q) || !in(q)) continue;
+        const uint32_t to = slot + uint32_t(q) * pitch;
 #pragma unroll
-        for (int k = 0; k < P; ++k)
-          v[k] = pack2(__uint_as_float(ld_shared_word(slot + uint32_t(2 * k) * pitch)),
-                       __uint_as_float(ld_shared_word(slot + uint32_t(2 * k + 1) * pitch)));
-      } else {
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-          const uint32_t w = ld_shared_word(slot + uint32_t(k) * pitch);
-          v[k] = pack2(widen_lo<T>(w), widen_hi<T>(w));
+        for (int j = 0; j < V; ++j) {
+          if (has(q, j)) continue;
+          for (int k = 0; k < arrays; ++k) {
+            if constexpr (B == 4) st_shared_word(to + uint32_t(k) * array + 4u * j, 0u);
+            else st_shared_half(to + uint32_t(k) * array + 2u * j, 0);
+          }
         }
       }
+    }
+  }
+  __device__ __forceinline__ void clear_outside(int q, uint64_t* v) const {
+    const uint32_t from = uint32_t(low(q)), n = uint32_t(count(q));
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      float lo, hi;
+      unpack2(v[j / 2], lo, hi);
+      v[j / 2] = pack2(uint32_t(j) - from < n ? lo : 0.0f, uint32_t(j + 1) - from < n ? hi : 0.0f);
+    }
+  }
+  template <bool kMask>
+  __device__ __forceinline__ void read(uint32_t slot, const void* p, uint64_t off, uint64_t (&v)[P]) const {
+    if constexpr (F == NORM_UNITS || F == NORM_CUT) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        act_widen2<T>(ld_shared(slot + uint32_t(q) * pitch), v + q * V / 2);
+        if (kMask && F == NORM_CUT && (cuts & 1u << q)) clear_outside(q, v + q * V / 2);
+      }
+    } else if constexpr (F == NORM_WORDS) {
+#pragma unroll
+      for (int k = 0; k < P; ++k)
+        v[k] = pack2(__uint_as_float(ld_shared_word(slot + uint32_t(2 * k) * pitch)),
+                     __uint_as_float(ld_shared_word(slot + uint32_t(2 * k + 1) * pitch)));
     } else {
       // of all units: they are whole words apart
       const uint32_t shift = (uint32_t(reinterpret_cast<uintptr_t>(p)) + uint32_t(off)) & 15u;
@@ -149,17 +194,21 @@ struct Columns {
 #pragma unroll
       for (int q = 0; q < Q; ++q)
         if (on && in(q)) st_stream_v4(to + unit(off, q), act_narrow2<T>(v + q * V / 2));
+    } else if constexpr (F == NORM_CUT) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        if (!on || !in(q)) continue;
+        const uint4 o = act_narrow2<T>(v + q * V / 2);
+        if (count(q) == V) st_stream_v4(to + unit(off, q), o);
+        else store_cut<T>(to + unit(off, q), o, low(q), high(q));
+      }
     } else if constexpr (F == NORM_WORDS) {
 #pragma unroll
       for (int k = 0; k < P; ++k) {
         float lo, hi;
         unpack2(v[k], lo, hi);
-        if constexpr (T == kF32) {
-          if (on && in(2 * k)) st_stream_u32(to + unit(off, 2 * k), __float_as_uint(lo));
-          if (on && in(2 * k + 1)) st_stream_u32(to + unit(off, 2 * k + 1), __float_as_uint(hi));
-        } else {
-          if (on && in(k)) st_stream_u32(to + unit(off, k), narrow_two<T>(lo, hi));
-        }
+        if (on && in(2 * k)) st_stream_u32(to + unit(off, 2 * k), __float_as_uint(lo));
+        if (on && in(2 * k + 1)) st_stream_u32(to + unit(off, 2 * k + 1), __float_as_uint(hi));
       }
     } else {
       const uint32_t place = t.lane & (t.lanes - 1);
@@ -177,29 +226,32 @@ struct Columns {
   __device__ __forceinline__ void params(const void* p, int type, uint64_t offset, float fill, float* f) const {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int n = count(q);
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[q * V + j] = j < n ? fill : 0.0f;
+      for (int j = 0; j < V; ++j) f[q * V + j] = has(q, j) ? fill : 0.0f;
       if (!p) continue;
-      if (F == NORM_UNITS) {
-        if constexpr (F == NORM_UNITS) {
-          if (n) param_load<V>(p, type, offset + at(q), f + q * V);
-        }
+      if constexpr (F == NORM_UNITS) {
+        if (in(q)) param_load<V>(p, type, offset + uint32_t(at(q)), f + q * V);
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (j < n) param_load<1>(p, type, offset + at(q) + j, f + q * V + j);
+          if (has(q, j)) param_load<1>(p, type, offset + uint32_t(at(q) + j), f + q * V + j);
       }
     }
   }
-  // v - mean where there is a column; the rest stays 0
+  // v - mean; where there is no column, 0 if kExact
+  template <bool kExact>
   __device__ __forceinline__ void center(float mean, uint64_t (&v)[P]) const {
-    if constexpr (F == NORM_UNITS) {
+    if constexpr (!kExact) {
+      const uint64_t m = both(-mean);
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = add2(v[k], m);
+    } else if constexpr (F == NORM_UNITS || F == NORM_CUT) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const uint64_t m = both(in(q) ? -mean : 0.0f);
 #pragma unroll
         for (int k = 0; k < V / 2; ++k) v[q * V / 2 + k] = add2(v[q * V / 2 + k], m);
+        if (F == NORM_CUT && (cuts & 1u << q)) clear_outside(q, v + q * V / 2);
       }
     } else {
       float f[E];
@@ -224,14 +276,14 @@ struct Columns {
     if constexpr (F == NORM_WORDS) {
 #pragma unroll
       for (int q = 0; q < Q; q += 4) {  // four blocks side by side
-        const uint64_t i[4] = {e + uint32_t(q) * step, e + uint32_t(q + 1) * step, e + uint32_t(q + 2) * step,
-                               e + uint32_t(q + 3) * step};
-        drop_keep_words<4, V>(run, i, keep + q * V);
+        const uint64_t i[4] = {e + uint32_t(q * step), e + uint32_t((q + 1) * step), e + uint32_t((q + 2) * step),
+                               e + uint32_t((q + 3) * step)};
+        drop_keep_words<4>(run, i, keep + q);
       }
     } else {
       uint64_t i[Q];
 #pragma unroll
-      for (int q = 0; q < Q; ++q) i[q] = e + uint32_t(q) * step;
+      for (int q = 0; q < Q; ++q) i[q] = e + uint32_t(q * step);
       drop_keep<Q, V, F == NORM_ANYWHERE>(run, i, keep);
     }
 #pragma unroll
@@ -295,11 +347,10 @@ __device__ __forceinline__ void scale_by(uint64_t (&v)[kPairs], const ParamSlot&
   }
 }
 
-// Stages of the ring: up to three while 512 threads an SM (what the registers
-// allow) still fit its shared memory.
+// Stages of the ring: two where 512 threads still fit an SM's shared memory.
 constexpr int kParamBytes = kElems * 4, kThreadBytes = 440;
 constexpr int ring_stages(int stage_bytes, int param_bytes) {
-  return 3 * stage_bytes + param_bytes <= kThreadBytes ? 3 : 2 * stage_bytes + param_bytes <= kThreadBytes ? 2 : 1;
+  return 2 * stage_bytes + param_bytes <= kThreadBytes ? 2 : 1;
 }
 
 struct Chosen {
@@ -325,10 +376,8 @@ Chosen choose_switches(const NormArgs& a) {
 }
 template <template <int, int, int, bool, bool> class Pick, int T>
 Chosen choose_type(const NormArgs& a, NormFit fit) {
-  if (fit == NORM_WORDS) return choose_switches<Pick, T, NORM_WORDS, FORM_ANY>(a);
-  if constexpr (T != kF32) {
-    if (fit == NORM_ANYWHERE) return choose_switches<Pick, T, NORM_ANYWHERE, FORM_ANY>(a);
-  }
+  if (fit == NORM_CUT) return choose_switches<Pick, T, NORM_CUT, FORM_ANY>(a);
+  if (fit != NORM_UNITS) return choose_switches<Pick, T, T == kF32 ? NORM_WORDS : NORM_ANYWHERE, FORM_ANY>(a);
   switch (norm_form(a)) {
     case FORM_BOTH: return choose_switches<Pick, T, NORM_UNITS, FORM_BOTH>(a);
     case FORM_ADD: return choose_switches<Pick, T, NORM_UNITS, FORM_ADD>(a);

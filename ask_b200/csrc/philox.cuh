@@ -176,22 +176,16 @@ __device__ __forceinline__ void drop_keep(const DropRun& r, const uint64_t (&i)[
     }
   }
 }
-// The same of runs of N = 1 or 2 elements, each within one block (i[u] is a
-// multiple of N): a block for each run.
-template <int kRuns, int N>
+// The same of single elements: a block for each.
+template <int kRuns>
 __device__ __forceinline__ void drop_keep_words(const DropRun& r, const uint64_t (&i)[kRuns], bool* keep) {
-  static_assert(N == 1 || N == 2, "part of a block");
   Philox w[kRuns];
   drop_words<kRuns, 1>(r, i, w);
 #pragma unroll
   for (int u = 0; u < kRuns; ++u) {
     const bool upper = i[u] & 2;
     const uint32_t a = upper ? w[u].c[2] : w[u].c[0], b = upper ? w[u].c[3] : w[u].c[1];
-    if constexpr (N == 1) keep[u] = ((i[u] & 1) ? b : a) >= r.threshold;
-    else {
-      keep[2 * u] = a >= r.threshold;
-      keep[2 * u + 1] = b >= r.threshold;
-    }
+    keep[u] = ((i[u] & 1) ? b : a) >= r.threshold;
   }
 }
 // N elements dropped and scaled.

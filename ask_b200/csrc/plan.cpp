@@ -25,6 +25,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <numeric>
 #include <sstream>
 #include <string>
 #include <vector>
@@ -933,8 +934,9 @@ uint64_t chunk_count(uint64_t groups, uint64_t units, uint64_t slots) {
 
 // The fit of a step's rows: `low` holds the low bits of every row port's address.
 NormFit norm_fit(const NormArgs& a, uint64_t low) {
-  const uint64_t bytes = a.cols * uint64_t(dtype_bytes(a.type)) | low;
-  return bytes % 16 == 0 ? NORM_UNITS : bytes % 4 == 0 ? NORM_WORDS : NORM_ANYWHERE;
+  if (low % 16 == 0 && a.cols * uint64_t(dtype_bytes(a.type)) % 16 == 0) return NORM_UNITS;
+  if (low % 16 == 0 && a.classes > 1) return NORM_CUT;
+  return a.type == kF32 ? NORM_WORDS : NORM_ANYWHERE;
 }
 
 // {"family": "block_norm" | "block_norm_grad", "dtype", "rows", "cols", "norm":
@@ -1017,7 +1019,7 @@ void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
   }
   in(a.drop.on, kI64, 2);
 
-  a.shape = norm_shape(cols, a.type, grad);
+  norm_layout(&a, grad);
   pl.block = a.shape.threads;
   int occ = 2;
   if (pl.device >= 0) {
@@ -1028,15 +1030,20 @@ void build_norm(ask_b200_plan& pl, const json::Value& r, bool grad) {
   if (pl.blocks_per_sm) occ = std::min(occ, pl.blocks_per_sm);
   const uint64_t slots = std::max<uint64_t>(1, uint64_t(pl.num_sms) * uint64_t(std::max(occ, 1)) / uint64_t(a.shape.ctas));
   const uint64_t teams = uint64_t(team_count(a.shape));
+  a.spread = a.classes / std::gcd(a.classes, uint32_t(teams));
+  if (grad && a.rows_per_group <= teams) a.spread = 1;  // a row a team
+  const uint64_t turn = teams * a.spread;  // rows at work on one stretch
+  const uint64_t stretches = std::max<uint64_t>(1, slots / a.spread);
   const std::string name = std::string(a.layer ? "layer_" : "rms_") + kTypeNames[a.type];
   if (!grad) {
     pl.kernel = "norm_rows_" + name;
-    pl.grid = int(std::max<uint64_t>(1, std::min<uint64_t>((a.rows + teams - 1) / teams, slots)) * uint64_t(a.shape.ctas));
+    pl.grid = int(std::max<uint64_t>(1, std::min<uint64_t>((a.rows + turn - 1) / turn, stretches)) * a.spread *
+                  uint64_t(a.shape.ctas));
     pl.launches = a.rows ? 1 : 0;
     return;
   }
   pl.kernel = "norm_grad_" + name;
-  a.chunks = uint32_t(chunk_count(a.groups, (a.rows_per_group + teams - 1) / teams, slots));
+  a.chunks = uint32_t(chunk_count(a.groups, (a.rows_per_group + turn - 1) / turn, stretches)) * a.spread;
   const uint64_t places = mul_checked(a.groups, a.chunks);
   if (places * uint64_t(a.shape.ctas) > uint64_t(INT32_MAX)) fail(ASK_B200_E_UNSUPPORTED, "too many gate groups");
   pl.grid = int(places * uint64_t(a.shape.ctas));

@@ -210,6 +210,20 @@ def test_block_norm_rows_off_the_units(device, dtype, params, cols, switch):
     run_norm(dtype, params, 12, cols, switch)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [4095, 5120, 7001, 8192])
+def test_block_norm_widest_ctas(device, dtype, cols):
+    """Layer norms with biases on the most threads a CTA has: what takes most registers and shared memory."""
+    run_norm(dtype, "f32", 18, cols, (True, True, True, True, True, 2, 0.1, 1.0))
+
+
+@pytest.mark.parametrize("dtype,cols", [("bf16", 4099), ("f16", 1002), ("f32", 2051), ("bf16", 45), ("f16", 257)])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_block_norm_teams_keep_their_place_of_a_unit(device, dtype, cols, groups):
+    """More rows than CTAs, off the units: a team meets rows of one alignment only."""
+    run_norm(dtype, "f32", 3 * (201 + 200000 // cols), cols, (False, True, True, True, False, groups, 0.1, 1.0))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 601, 5000])
 @pytest.mark.parametrize("cols", [96, 1000])
 def test_block_norm_row_counts(device, rows, cols):
