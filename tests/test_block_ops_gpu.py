@@ -278,6 +278,34 @@ def test_block_norm_nan_and_inf_stay_in_their_row(device):
     assert np.isnan(host(h, (rows, cols))).any(1).tolist() == bad.tolist()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [45, 301, 1001, 4099])
+@pytest.mark.parametrize("skew", [0, 1])
+@pytest.mark.parametrize("layer", [False, True])
+def test_block_norm_neighbours_of_nan(device, dtype, cols, skew, layer):
+    """Rows that share a 16-byte unit with a NaN or an infinity are not touched by it, forward or backward."""
+    rng = np.random.default_rng(cols)
+    rows = 11
+    bad = {2: 0, 5: cols - 1, 7: 0, 8: cols - 1}
+    mark = lambda v: [v.__setitem__((r, c), np.nan if r != 8 else np.inf) for r, c in bad.items()]  # noqa: E731
+    x, y, dh, du, h = (rounded(rng, (rows, cols), dtype) for _ in range(5))
+    w = np.ones(cols)
+    norm = "layer" if layer else "rms"
+    args = dict(norm=norm)
+    mark(y)
+    hh, u = launch(R.block_norm(dtype, rows, cols, **args), [dev(x, dtype, skew), dev(y, dtype, skew), dev(w, "f32"), dev(w, "f32")], skew)[:2]
+    want = [r in bad for r in range(rows)]
+    assert (~np.isfinite(host(hh, (rows, cols)))).any(1).tolist() == want
+    assert (~np.isfinite(host(u, (rows, cols)))).any(1).tolist() == want
+    y = rounded(rng, (rows, cols), dtype)
+    mark(du), mark(dh)
+    stats = dev(np.ones((rows, 2 if layer else 1)), "f32")
+    dx, dy = launch(R.block_norm_grad(dtype, rows, cols, **args),
+                    [dev(v, dtype, skew) for v in (dh, du, h, y)] + [dev(w, "f32"), dev(w, "f32"), stats, stats], skew)[:2]
+    assert (~np.isfinite(host(dx, (rows, cols)))).any(1).tolist() == want
+    assert (~np.isfinite(host(dy, (rows, cols)))).any(1).tolist() == want
+
+
 # ---- bucketed-bias softmax -----------------------------------------------------------------------
 def run_softmax(dtype, shape, thresholds, both=True, scale=1.0, causal=False, lengths=None, offsets=None, p=0.0,
                 table_dtype="f32", skew=0, grad=True, s=None, seed=0):
