@@ -197,7 +197,7 @@ void norm_layout(NormArgs* a, bool grad) {
   a->classes = 1;
   a->shape = shape_of(a->cols, grad);
   if (a->cols % v == 0) return;
-  // Rows off the units go by cut units (bf16 [33520, 1001] 93 us, and 146 shifted out
+  // Rows off the units go by cut units (bf16 [33520, 1001] 87 us, and 146 shifted out
   // of neighbouring words; f32 107, and 207 word by word), unless the unit more that a
   // row may spread over needs threads that halve the teams an SM holds (gradient
   // of bf16 [8191, 4095] 222 us, and 190 shifted; of 511 columns 235 and 187; with
