@@ -239,7 +239,7 @@ struct Units {
     return key(r, u) < r.visible && (kEven || key(r, u) > -V);
   }
 
-  // `units` lie in the tensor whole: all rows but its last one's, of an aligned tensor
+  // `units`: the row's units lie in the tensor whole
   __device__ __forceinline__ void fetch(const void* p, const RowView& r, bool units, int u, uint32_t slot) const {
     if (!seen(r, u)) return;
     const char* from = static_cast<const char*>(p) + offset(r, u);

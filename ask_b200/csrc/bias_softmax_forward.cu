@@ -20,7 +20,6 @@ __global__ void __launch_bounds__(kSmall ? kWarpTeamThreads : kTeamThreads, kSma
   const uint32_t pitch = blockDim.x * 16, ring = shared_address(dynamic) + threadIdx.x * 16;
   float* const copies = reinterpret_cast<float*>(dynamic + a.ring_rows * row_words<T, E>() * blockDim.x);
   float* const window = copies + (a.window_copies ? Lut<V>::words(win) : 0);
-  const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
@@ -29,7 +28,7 @@ __global__ void __launch_bounds__(kSmall ? kWarpTeamThreads : kTeamThreads, kSma
   uint64_t index = 0;
   auto fetch = [&](uint32_t slot) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) units.fetch(a.s, row, a.aligned && rows.index != last_row, u, slot + uint32_t(u) * pitch);
+    for (int u = 0; u < U; ++u) units.fetch(a.s, row, rows.index < a.whole_rows, u, slot + uint32_t(u) * pitch);
   };
   bool on = rows.left > 0;
   if (on) {

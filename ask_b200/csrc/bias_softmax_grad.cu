@@ -24,7 +24,6 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   float* const window = copies + (a.window_copies ? Lut<V>::words(win) : 0);
   float* const sums = window + win.words();  // the teams' windows
   const uint32_t mine = shared_address(sums + int(t.index) * win.words());
-  const uint64_t last_row = a.batch * a.heads * a.queries - 1;
   const Units<T, kEven> units(a, t);
   pdl_enter();
   team_start(t);
@@ -32,7 +31,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   RowView row{};
   float row_lse = 0.0f;
   auto fetch = [&](uint32_t slot) {
-    const bool whole = a.aligned && rows.index != last_row;
+    const bool whole = rows.index < a.whole_rows;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       units.fetch(a.s, row, whole, u, slot + uint32_t(2 * u) * pitch);

@@ -285,6 +285,7 @@ struct BiasSoftmaxArgs {
   float* dtable;   // gradient, [buckets, heads]
   float* partial;  // gradient: [heads * chunks * ctas][buckets]
   uint64_t batch, queries;
+  uint64_t whole_rows;  // rows below this one may be read by whole units: those end inside the tensor
   uint32_t heads, keys, chunks;  // chunks of a head's (batch, query) pairs
   uint32_t buckets;
   float scale;

@@ -1112,6 +1112,11 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
   a.offsets = offsets ? reinterpret_cast<const int*>(1) : nullptr;
 
   a.aligned = 1;  // until a launch sees the addresses
+  // Row r's last unit ends at (r + 1) keys rounded up to a unit; it lies in the tensor
+  // if (r + 1) keys is within the tensor's whole units.  Rows of fewer keys than a unit
+  // has elements can reach past the end from several rows before the last.
+  const uint64_t v = a.type == kF32 ? 4 : 8;
+  a.whole_rows = keys ? n / v * v / keys : 0;
   a.shape = bias_softmax_shape(keys, rows, a.type, grad, pl.num_sms);
   if (a.shape.threads > kBiasMaxThreads)
     fail(ASK_B200_E_UNSUPPORTED, "rows that start inside a 16-byte unit take at most " +
@@ -1195,6 +1200,8 @@ std::string describe(const ask_b200_plan& pl) {
   if (pl.family == FAM_ELEMENTWISE || pl.family == FAM_REDUCE)
     o << ",\"specialized\":" << (pl.spec ? "true" : "false") << ",\"registers\":" << int(pl.prog.n_regs);
   if (pl.family == FAM_SCATTER) o << ",\"pre_copy\":{\"input\":0,\"output\":0}";
+  if (pl.family == FAM_BIAS_SOFTMAX || pl.family == FAM_BIAS_SOFTMAX_GRAD)
+    o << ",\"whole_unit_rows\":" << pl.bias.whole_rows;
   o << ",\"port_map\":[";
   size_t arg = 0;
   auto port = [&](const PortInfo& p, const char* kind, size_t k) {
@@ -1464,6 +1471,7 @@ void launch_plan(const ask_b200_plan& pl, const uint64_t* ports, uint64_t scratc
       if (a.offsets) a.offsets = reinterpret_cast<const int*>(*at++);
       if (a.drop.on) a.seed = reinterpret_cast<const int64_t*>(*at++);
       a.aligned = a.aligned && aligned16(*at);
+      if (!a.aligned) a.whole_rows = 0;
       a.out = reinterpret_cast<void*>(*at++);
       if (grad) a.dtable = reinterpret_cast<float*>(*at);
       else a.lse = reinterpret_cast<float*>(*at);

@@ -175,3 +175,19 @@ def test_reference_gradients_against_differences():
             args = lambda t: [s + t * v if k == 0 else s, table + t * v if k == 1 else table]  # noqa: E731
             num = (loss(*args(1e-5)) - loss(*args(-1e-5))) / 2e-5
             assert abs(num - (g * v).sum()) <= 1e-7 * (1 + np.abs(g * v).sum())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("make", [R.bias_softmax, R.bias_softmax_grad])
+def test_whole_units_end_inside_the_scores(dtype, make):
+    """A row of scores is copied by whole aligned 16-byte units where each of them ends inside the tensor: with fewer
+    keys than a unit has elements, several rows before the last reach past its end."""
+    v = 4 if dtype == "f32" else 8
+    for keys in list(range(0, 18)) + [45, 1021]:
+        for batch, heads, queries in [(1, 1, 1), (1, 1, 5), (2, 3, 5), (1, 2, 8), (3, 1, 11)]:
+            rows = batch * heads * queries
+            whole = ask_b200.Plan(make(dtype, batch, heads, queries, keys, [1, 2]), -1).describe()["whole_unit_rows"]
+            assert 0 <= whole <= rows
+            for r in range(rows):
+                end = -(-(r + 1) * keys // v) * v  # of the row's last unit, in elements
+                assert (r < whole) == (end <= rows * keys and keys > 0), (keys, rows, r)

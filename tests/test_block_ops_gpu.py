@@ -375,6 +375,28 @@ def test_bias_softmax_single_tokens(device, dtype, keys):
     run_softmax(dtype, (batch, heads, 1, keys), TH1, False, 0.125, False, lengths, [n - 1 for n in lengths])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("keys", [1, 2, 3, 5, 6])
+@pytest.mark.parametrize("shape", [(1, 1, 5), (2, 3, 7), (3, 5, 101)])
+def test_bias_softmax_fewer_keys_than_a_unit(device, dtype, keys, shape):
+    """Several rows before the last end in the tensor's last partial unit; the tensors are exactly as long as they are."""
+    rng = np.random.default_rng(keys)
+    shape = (*shape, keys)
+    s, dp, table = rounded(rng, shape, dtype), rounded(rng, shape, dtype), rounded(rng, (6, shape[1]), "f32")
+    tight = lambda a, t: torch.from_numpy(a.reshape(-1)).to(TORCH[t]).cuda()  # noqa: E731
+    p, lse = launch(R.bias_softmax(dtype, *shape, [1, 2]), [tight(s, dtype), tight(table, "f32")])
+    prob, ptol, lse64, ltol = ref.bias_softmax(s, table, [1, 2], True, 1.0, False, None, None, None)
+    close(host(p, shape), prob, ptol + ref.HALF_ULP[dtype] * (prob + ptol) + ref.TINY[dtype], "p")
+    close(host(lse, lse64.shape), lse64, ltol + ref.U * np.abs(lse64), "lse")
+    lse32 = lse64.astype(np.float32)
+    ds, dt = launch(R.bias_softmax_grad(dtype, *shape, [1, 2]),
+                    [tight(s, dtype), tight(dp, dtype), tight(lse32, "f32"), tight(table, "f32")])
+    gs, gtol, gt, ttol = ref.bias_softmax_grad(s, dp, lse32.astype(np.float64), table, [1, 2], True, 1.0, False, None,
+                                               None, None)
+    close(host(ds, shape), gs, gtol + ref.HALF_ULP[dtype] * (np.abs(gs) + gtol) + ref.TINY[dtype], "ds")
+    close(host(dt, gt.shape), gt, ttol + ref.U * np.abs(gt), "dtable")
+
+
 def test_bias_softmax_longest_rows(device):
     run_softmax("bf16", (1, 2, 1, 131072), TH, offsets=[131071])
 
