@@ -100,7 +100,9 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     }
     float dot[1] = {sum2(add2(s2, s3))};
     team_sum<1>(t, sh, int(turn & 1u), dot);
-    if (a.shape.warp_teams) __syncwarp();  // the lanes' adds of the row before are done
+    // The lanes' adds of the row before are done: a team of several warps has met at
+    // its barrier, shuffles alone order no memory.
+    __syncwarp();
     // masked keys hold P = 0 already, unless the sum is a NaN or infinite
     const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
     if (!two && on) fetch(ring);

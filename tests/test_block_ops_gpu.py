@@ -397,6 +397,26 @@ def test_bias_softmax_fewer_keys_than_a_unit(device, dtype, keys, shape):
     close(host(dt, gt.shape), gt, ttol + ref.U * np.abs(gt), "dtable")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("keys", [30, 200, 253])
+@pytest.mark.parametrize("thresholds", [[1, 2, 4, 60], R.bucket_thresholds(64, 1600, True)])
+def test_bias_softmax_one_warp_takes_many_rows(device, dtype, keys, thresholds):
+    """CTAs of one warp that take several rows each: every row adds to the window's sums where another lane did before."""
+    shape = (2, 4, 130, keys)
+    rng = np.random.default_rng(keys)
+    recipe = dict(R.bias_softmax_grad(dtype, *shape, thresholds), blocks_per_sm=1)
+    where = ask_b200.Plan(recipe, device=0).describe()["launch"]
+    assert where["block"][0] == 32 and where["grid"][0] < 2 * 4 * 130 // 3
+    table = rounded(rng, (2 * len(thresholds) + 2, shape[1]), "f32")
+    s, dp = rounded(rng, shape, dtype), rounded(rng, shape, dtype)
+    lse = ref.bias_softmax(s, table, thresholds, True, 1.0, False, None, None, None)[2].astype(np.float32)
+    ds, dt = launch(recipe, [dev(s, dtype), dev(dp, dtype), dev(lse, "f32"), dev(table, "f32")])
+    gs, gtol, gt, ttol = ref.bias_softmax_grad(s, dp, lse.astype(np.float64), table, thresholds, True, 1.0, False, None,
+                                               None, None)
+    close(host(ds, shape), gs, gtol + ref.HALF_ULP[dtype] * (np.abs(gs) + gtol) + ref.TINY[dtype], "ds")
+    close(host(dt, gt.shape), gt, ttol + ref.U * np.abs(gt), "dtable")
+
+
 def test_bias_softmax_longest_rows(device):
     run_softmax("bf16", (1, 2, 1, 131072), TH, offsets=[131071])
 
