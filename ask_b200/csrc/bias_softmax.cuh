@@ -5,8 +5,9 @@
 //   over the keys k < length[batch] (and k <= pos when causal);
 //   p = D(exp(l - lse)),  lse = log sum exp l,  D dropout; a row without keys
 //   gives zeros and lse = -inf.
-//   Gradient: P = exp(l - lse), d = D(dp), dl = P (d - sum P d), ds = scale dl,
-//   dtable[b, head] = sum of dl where the bucket is b.
+//   Gradient: P = exp(l - lse), divided by its sum where lse is too coarse to carry
+//   that, d = D(dp), dl = P (d - sum P d), ds = scale dl, dtable[b, head] = sum of dl
+//   where the bucket is b.
 //
 // bucket(rel): the number of thresholds that are at most the distance |rel|
 // (bidirectional; the buckets of rel > 0 follow those of rel <= 0) or

@@ -6,15 +6,26 @@
 // behind the team's reduction, so sums have one order and no atomics.
 #include "bias_softmax.cuh"
 
+#include <type_traits>
+
 namespace askb {
 
 namespace {
+
+// lse in 32 bits carries a row's sum only so well: its rounding moves P by half a unit
+// in lse's last place, 2^-18 below this magnitude, 0.2% at -65504, and where a whole row
+// is at the lowest f32, as masks of that value leave it, every key had P = 1.  From
+// here on P is divided by its sum over the row.  The loop's body is there twice for
+// it: dividing every row took 268 us (the registers that add P beside P d spill), a
+// branch within the body 236, this 234, and no division 233 (bf16 [8, 16, 1024, 1024],
+// ragged, with dropout).
+constexpr float kCoarseLse = 128.0f;
 
 template <int T, int E, bool kDrop, bool kEven>
 __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const __grid_constant__ BiasSoftmaxArgs a) {
   constexpr int V = act_vec<T>(), U = E / V, H = V / 2;
   extern __shared__ uint4 dynamic[];
-  __shared__ TeamRecords<1> sh;
+  __shared__ TeamRecords<1> sh, sh_total;
   __shared__ float ends[2][kTeamThreads / 32];
   const Team t = team_of(a.shape);
   const Window<V> win(a);
@@ -70,77 +81,100 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
     copy_async_commit();
     if (two) copy_async_wait<1>();
     else copy_async_wait<0>();
-    uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
+    const bool coarse = here && fabsf(base) >= kCoarseLse;  // the warps of a team agree: they hold the same row
+    auto work = [&](auto coarse_rows) {
+      uint64_t p[U][H], d[U][H], s2 = 0, s3 = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
-      act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
-      units.logits(r, win, lut, scale, u, p[u]);
-      if (!units.all_whole(r, u)) {
-        units.mask(r, u, kNegInf, p[u]);
-        units.mask(r, u, 0.0f, d[u]);
-      }
-      if (kDrop && units.any_seen(r, u)) {
-        const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
-        bool keep[V];
-        drop_keep<1, V>(run, i, keep);
-#pragma unroll
-        for (int j = 0; j < H; ++j) {
-          float lo, hi;
-          unpack2(d[u][j], lo, hi);
-          d[u][j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
+      for (int u = 0; u < U; ++u) {
+        act_widen2<T>(ld_shared(slot + uint32_t(2 * u) * pitch), p[u]);
+        act_widen2<T>(ld_shared(slot + uint32_t(2 * u + 1) * pitch), d[u]);
+        units.logits(r, win, lut, scale, u, p[u]);
+        if (!units.all_whole(r, u)) {
+          units.mask(r, u, kNegInf, p[u]);
+          units.mask(r, u, 0.0f, d[u]);
         }
-      }
-      exp_minus<H>(p[u], both(-base));
-#pragma unroll
-      for (int j = 0; j < H; j += 2) {
-        s2 = fma2(p[u][j], d[u][j], s2);
-        s3 = fma2(p[u][j + 1], d[u][j + 1], s3);
-      }
-    }
-    float dot[1] = {sum2(add2(s2, s3))};
-    team_sum<1>(t, sh, int(turn & 1u), dot);
-    // The lanes' adds of the row before are done: a team of several warps has met at
-    // its barrier, shuffles alone order no memory.
-    __syncwarp();
-    // masked keys hold P = 0 already, unless the sum is a NaN or infinite
-    const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
-    if (!two && on) fetch(ring);
-    // dl = P (D(dp) - sum): the dropout's scale enters here
-    const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint4 o = make_uint4(0u, 0u, 0u, 0u);
-      if (units.any_seen(r, u)) {
-        uint64_t* x = p[u];
-#pragma unroll
-        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
-        if (odd) units.mask(r, u, 0.0f, x);
-        const int rel = units.key(r, u) - r.pos;
-        const bool near = units.any_near(r, win, u);
-        if (!near || rel >= win.hi || rel + V - 1 <= -win.w) {
-          uint64_t v = x[0];
-#pragma unroll
-          for (int j = 1; j < H; ++j) v = add2(v, x[j]);
-          const float f = here ? sum2(v) : 0.0f;
-          left += rel >= win.hi ? 0.0f : f;
-          right += rel >= win.hi ? f : 0.0f;
-        } else if (here) {
-          const Places<V> at(mine, win.place(rel));
+        if (kDrop && units.any_seen(r, u)) {
+          const uint64_t i[1] = {units.offset(r, u) / dtype_bytes(T)};
+          bool keep[V];
+          drop_keep<1, V>(run, i, keep);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
             float lo, hi;
-            unpack2(x[j], lo, hi);
-            st_shared_f32(at(2 * j), ld_shared_f32(at(2 * j)) + lo);
-            st_shared_f32(at(2 * j + 1), ld_shared_f32(at(2 * j + 1)) + hi);
+            unpack2(d[u][j], lo, hi);
+            d[u][j] = pack2(keep[2 * j] ? lo : 0.0f, keep[2 * j + 1] ? hi : 0.0f);
           }
         }
+        exp_minus<H>(p[u], both(-base));
 #pragma unroll
-        for (int j = 0; j < H; ++j) x[j] = mul2(x[j], scale);
-        o = act_narrow2<T>(x);
+        for (int j = 0; j < H; j += 2) {
+          s2 = fma2(p[u][j], d[u][j], s2);
+          s3 = fma2(p[u][j + 1], d[u][j + 1], s3);
+        }
       }
-      if (here) units.store(a, r, u, o);
-    }
+      float dot[1] = {sum2(add2(s2, s3))};
+      team_sum<1>(t, sh, int(turn & 1u), dot);
+      if constexpr (decltype(coarse_rows)::value) {
+        s2 = s3 = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < H; j += 2) {
+            s2 = add2(s2, p[u][j]);
+            s3 = add2(s3, p[u][j + 1]);
+          }
+        float total[1] = {sum2(add2(s2, s3))};
+        team_sum<1>(t, sh_total, int(turn & 1u), total);
+        const float over = !coarse ? 1.0f : total[0] == 0.0f ? 0.0f : __frcp_rn(total[0]);
+        dot[0] *= over;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < H; ++j) p[u][j] = mul2(p[u][j], both(over));
+      }
+      // The lanes' adds of the row before are done: a team of several warps has met at
+      // its barrier, shuffles alone order no memory.
+      __syncwarp();
+      // masked keys hold P = 0 already, unless the sum is a NaN or infinite
+      const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
+      if (!two && on) fetch(ring);
+      // dl = P (D(dp) - sum): the dropout's scale enters here
+      const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+        if (units.any_seen(r, u)) {
+          uint64_t* x = p[u];
+#pragma unroll
+          for (int j = 0; j < H; ++j) x[j] = mul2(x[j], fma2(d[u][j], by, minus));
+          if (odd) units.mask(r, u, 0.0f, x);
+          const int rel = units.key(r, u) - r.pos;
+          const bool near = units.any_near(r, win, u);
+          if (!near || rel >= win.hi || rel + V - 1 <= -win.w) {
+            uint64_t v = x[0];
+#pragma unroll
+            for (int j = 1; j < H; ++j) v = add2(v, x[j]);
+            const float f = here ? sum2(v) : 0.0f;
+            left += rel >= win.hi ? 0.0f : f;
+            right += rel >= win.hi ? f : 0.0f;
+          } else if (here) {
+            const Places<V> at(mine, win.place(rel));
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              float lo, hi;
+              unpack2(x[j], lo, hi);
+              st_shared_f32(at(2 * j), ld_shared_f32(at(2 * j)) + lo);
+              st_shared_f32(at(2 * j + 1), ld_shared_f32(at(2 * j + 1)) + hi);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < H; ++j) x[j] = mul2(x[j], scale);
+          o = act_narrow2<T>(x);
+        }
+        if (here) units.store(a, r, u, o);
+      }
+    };
+    if (__any_sync(0xffffffffu, coarse)) work(std::true_type{});
+    else work(std::false_type{});
   }
   // fold the windows by bucket
 #pragma unroll

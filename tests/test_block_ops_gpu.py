@@ -472,6 +472,44 @@ def test_bias_softmax_extreme_scores(device):
         assert (ds[0] == 0).all() and np.isfinite(ds).all() and (ds[:, 30:] == 0).all() and bool(torch.isfinite(dt).all())
 
 
+def true_gradient(l, seen, dp, ids, buckets):
+    """Of softmax over the seen keys, from the scores alone: dl and its sums by bucket, in 64 bits."""
+    e = np.where(seen, np.exp(l - np.where(seen, l, -np.inf).max(3, keepdims=True)), 0)
+    p = e / e.sum(3, keepdims=True)
+    dl = p * (dp - (p * dp).sum(3, keepdims=True))
+    mag = p * (np.abs(dp) + (p * np.abs(dp)).sum(3, keepdims=True))
+    dt, dtmag = np.zeros((buckets, l.shape[1])), np.zeros((buckets, l.shape[1]))
+    for h in range(l.shape[1]):
+        np.add.at(dt[:, h], ids, dl[:, h])
+        np.add.at(dtmag[:, h], ids, mag[:, h])
+    return dl, mag, dt, dtmag
+
+
+@pytest.mark.parametrize("dtype,low,step", [("f32", -1e6, 0.25), ("f32", float(np.finfo(np.float32).min), 0.0),
+                                            ("f32", -2.0 ** 24, 1.0), ("f16", -65504.0, 0.0), ("f16", -60000.0, 32.0),
+                                            ("bf16", -3.3895e38, 0.0), ("bf16", 1e6, 0.0)])
+@pytest.mark.parametrize("shape", [(2, 3, 7, 40), (3, 4, 200, 100), (2, 1, 5, 3000)])
+def test_bias_softmax_gradient_of_rows_far_from_zero(device, dtype, low, step, shape):
+    """Rows whose scores share a large offset, as masks of the type's lowest value leave them: the row's lse, rounded to
+    32 bits, says little of its sum, and the gradient is still that of the softmax that the forward pass gave."""
+    rng = np.random.default_rng(3)
+    far = rng.random(shape[:3]) < 0.5
+    s = np.where(far[..., None], low + step * rng.integers(0, 8, shape), rng.standard_normal(shape))
+    s = torch.from_numpy(s).to(TORCH[dtype]).double().numpy()
+    dp = rounded(rng, shape, dtype)
+    lengths = [shape[3]] + [shape[3] // 2 + 1] * (shape[0] - 1)
+    table = np.zeros((2 * len(TH) + 2, shape[1]))
+    at = [dev(s, dtype), dev(table, "f32"), dev(np.array(lengths), "i32")]
+    p, lse = launch(R.bias_softmax(dtype, *shape, TH, lengths=True), at)
+    ds, dt = launch(R.bias_softmax_grad(dtype, *shape, TH, lengths=True), [at[0], dev(dp, dtype), lse, at[1], at[2]])
+    seen, _, ids = ref.masks_and_bias(shape, table, TH, True, False, lengths, None)
+    dl, mag, want, wantmag = true_gradient(s, seen, np.where(seen, dp, 0), ids, len(table))
+    # the scores are the logits, exactly; l - lse is at most some 20 off the exponents that count, and errs by C u
+    tol = 2 * ref.C * ref.U * mag + 2.0 ** -120
+    close(host(ds, shape), dl, tol + ref.HALF_ULP[dtype] * (np.abs(dl) + tol) + ref.TINY[dtype], "ds")
+    close(host(dt, want.shape), want, (2 * ref.C + ref.C + shape[0] * shape[2]) * ref.U * wantmag + 2.0 ** -100, "dtable")
+
+
 def test_bias_softmax_no_keys_and_no_rows(device):
     p, lse = launch(R.bias_softmax("f32", 2, 3, 4, 0, TH), [dev(np.zeros(0), "f32"), dev(np.zeros((32, 3)), "f32")])
     assert p.numel() == 0 and bool((lse == -math.inf).all())
