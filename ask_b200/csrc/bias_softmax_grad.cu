@@ -134,11 +134,12 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
       // The lanes' adds of the row before are done: a team of several warps has met at
       // its barrier, shuffles alone order no memory.
       __syncwarp();
-      // masked keys hold P = 0 already, unless the sum is a NaN or infinite
-      const bool odd = __any_sync(0xffffffffu, here && !(fabsf(dot[0]) <= 3.4e38f));
-      if (!two && on) fetch(ring);
       // dl = P (D(dp) - sum): the dropout's scale enters here
-      const uint64_t by = both(drop_scale), minus = both(-dot[0] * drop_scale);
+      const float minus_sum = -dot[0] * drop_scale;
+      // masked keys hold P = 0 already, unless what it meets is a NaN or infinite
+      const bool odd = __any_sync(0xffffffffu, here && !(fabsf(minus_sum) <= 3.4e38f));
+      if (!two && on) fetch(ring);
+      const uint64_t by = both(drop_scale), minus = both(minus_sum);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         uint4 o = make_uint4(0u, 0u, 0u, 0u);

@@ -510,6 +510,23 @@ def test_bias_softmax_gradient_of_rows_far_from_zero(device, dtype, low, step, s
     close(host(dt, want.shape), want, (2 * ref.C + ref.C + shape[0] * shape[2]) * ref.U * wantmag + 2.0 ** -100, "dtable")
 
 
+@pytest.mark.parametrize("keys", [40, 45, 700])
+def test_bias_softmax_gradient_overflow_stays_out_of_masked_places(device, keys):
+    """Rows whose sums overflow once the dropout's scale is on them (three of five keys kept): masked keys still get zeros, buckets that only they
+    could reach too."""
+    shape = (1, 2, 3, keys)
+    dp = np.full(shape, 3e38)
+    lengths, seed = dev(np.array([5]), "i32"), dev(np.array([99, 12]), "i64")
+    th = list(range(1, 256))
+    table = np.zeros((512, 2))
+    at = [dev(np.zeros(shape), "f32"), dev(table, "f32"), lengths, seed]
+    _, lse = launch(R.bias_softmax("f32", *shape, th, lengths=True, dropout=0.5), at)
+    ds, dt = launch(R.bias_softmax_grad("f32", *shape, th, lengths=True, dropout=0.5), [at[0], dev(dp, "f32"), lse] + at[1:])
+    assert (host(ds, shape)[..., 5:] == 0).all()
+    dt = host(dt, (512, 2))
+    assert (dt[256 + 5:] == 0).all() and (dt[3:256] == 0).all()  # only distances -2 .. 4 are seen
+
+
 def test_bias_softmax_no_keys_and_no_rows(device):
     p, lse = launch(R.bias_softmax("f32", 2, 3, 4, 0, TH), [dev(np.zeros(0), "f32"), dev(np.zeros((32, 3)), "f32")])
     assert p.numel() == 0 and bool((lse == -math.inf).all())
