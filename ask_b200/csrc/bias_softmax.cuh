@@ -183,8 +183,9 @@ struct Rows {
     length = int(a.keys);
     place = 0;
     if (a.lengths) length = max(min(__ldg(a.lengths + b), length), 0);
-    // far positions meet only the window's ends, whatever their distance
-    if (a.offsets) place = max(min(__ldg(a.offsets + b), (1 << 30) - 1), -(1 << 30));
+    // far positions meet only the window's ends, whatever their distance; the upper bound
+    // leaves a unit that begins before its row within 32 bits of the last query
+    if (a.offsets) place = max(min(__ldg(a.offsets + b), (1 << 30) - 16), -(1 << 30));
     index = (uint64_t(b) * a.heads + head) * a.queries + q;
   }
   __device__ __forceinline__ void next(const BiasSoftmaxArgs& a) {

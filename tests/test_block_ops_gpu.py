@@ -527,6 +527,18 @@ def test_bias_softmax_gradient_overflow_stays_out_of_masked_places(device, keys)
     assert (dt[256 + 5:] == 0).all() and (dt[3:256] == 0).all()  # only distances -2 .. 4 are seen
 
 
+def test_bias_softmax_last_positions(device):
+    """2^30 queries behind the largest offset: the distance of a row's unit to its query stays within 32 bits."""
+    n = 2 ** 30
+    s = torch.zeros(n, dtype=torch.float16, device="cuda")
+    p, lse = torch.empty_like(s), torch.empty(n, device="cuda")
+    table = dev(np.array([1.0, 2.0, 3.0, 4.0, 5.0, 6.0]), "f32")  # [6 buckets, 1 head]
+    ask_b200.Plan(R.bias_softmax("f16", 1, 1, n, 1, [1, 2], offsets=True), 0).launch(
+        [s, table, dev(np.array([2 ** 31 - 1]), "i32")], [p, lse], None, torch.cuda.current_stream())
+    wrong = [int((p != 1).sum()), int(((lse - 3.0).abs() > ref.C * ref.U * 3).sum())]
+    assert wrong == [0, 0]
+
+
 def test_bias_softmax_no_keys_and_no_rows(device):
     p, lse = launch(R.bias_softmax("f32", 2, 3, 4, 0, TH), [dev(np.zeros(0), "f32"), dev(np.zeros((32, 3)), "f32")])
     assert p.numel() == 0 and bool((lse == -math.inf).all())
