@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTeamThreads) bias_softmax_grad_kernel(const _
   }
 }
 
-// dtable[b, head]: a warp adds the head's CTAs in order of their chunks.
+// dtable[b, head]: a warp (kBiasJoinThreads) adds the head's CTAs in order of their chunks.
 __global__ void __launch_bounds__(256) bias_table_join_kernel(const float* __restrict__ partial, float* __restrict__ dtable,
                                                               uint32_t heads, uint32_t buckets, uint32_t chunks,
                                                               uint32_t ctas) {

@@ -249,6 +249,7 @@ struct NormArgs {
   TeamShape shape;
 };
 constexpr int kNormMaxCols = 32768;
+constexpr int kNormJoinThreads = 16;  // that join one column's sums (gradient)
 void norm_layout(NormArgs* a, bool grad);  // sets shape and classes
 // How rows are read: as whole 16-byte units; as the units of the aligned tensor,
 // cut at the rows' ends; else f32 by words and 16-bit types from anywhere.
@@ -275,6 +276,7 @@ constexpr int kBiasMaxThresholds = 255;
 constexpr int kBiasMaxDistance = 4096;
 constexpr uint64_t kBiasMaxKeys = 131072;
 constexpr int kBiasMaxThreads = 512;  // of a CTA
+constexpr int kBiasJoinThreads = 32;  // that join one entry of the table's gradient
 struct BiasSoftmaxArgs {
   const void *s, *dp, *table;
   const float* lse_in;

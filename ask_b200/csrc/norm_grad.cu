@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_grad_kernel(const __grid_co
 // and adding what they found in warp order.  A CTA row (blockIdx.y) has one task:
 // a group's gate gradient, the post norm's parameters (gate times the groups'
 // sums), or the pre norm's.
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = kNormJoinThreads;
 
 __global__ void __launch_bounds__(32 * kJoinWarps) norm_grad_join_kernel(const __grid_constant__ NormArgs a,
                                                                          const NormSums kinds, const uint32_t gate_rows) {

@@ -404,8 +404,7 @@ void assign_registers(Program& p) {
 const char* const kFamilyNames[] = {"elementwise", "reduce",     "gather",          "scatter_add",  "softmax",
                                     "dropout",     "block_norm", "block_norm_grad", "bias_softmax", "bias_softmax_grad"};
 
-// The families whose kernels give a row (or a unit of elements) to threads in
-// their own way: their plans carry the CTA size in `block`.
+// The families whose plans carry the CTA size in `block`.
 bool row_family(int family) { return family >= FAM_SOFTMAX; }
 
 uint64_t checked_count(const json::Value& v, const char* what) {
@@ -1140,6 +1139,74 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
   if (grad && rows) pl.scratch = size_t(ctas * a.buckets * sizeof(float));
 }
 
+// What cuda_lowering (below) reports for the training-block families: a group for
+// each kind of outputs.  What is made row by row counts rows and a row's
+// threads, as the fused softmax does; sums over rows (parameter gradients, the bias
+// table's) count their elements and the threads that join one.  Reductions that
+// follow one another are passes of their own.
+struct OutputGroup {
+  std::vector<size_t> outputs;
+  uint64_t count, threads;
+};
+std::vector<OutputGroup> block_groups(const ask_b200_plan& pl, int* reductions) {
+  std::vector<OutputGroup> groups;
+  auto put = [&](size_t k, uint64_t count, uint64_t threads) {
+    if (pl.outputs[k].elements == 0) return;
+    if (groups.empty() || groups.back().count != count || groups.back().threads != threads)
+      groups.push_back({{}, count, threads});
+    groups.back().outputs.push_back(k);
+  };
+  const auto row_threads = [](const TeamShape& s) {
+    return uint64_t(s.warp_teams ? s.warp_teams : s.team_threads * s.ctas);
+  };
+  *reductions = 0;
+  if (pl.family == FAM_DROPOUT) {
+    put(0, pl.drop.count, 1);
+  } else if (pl.family == FAM_BLOCK_NORM || pl.family == FAM_BLOCK_NORM_GRAD) {
+    const NormArgs& a = pl.norm;
+    const bool grad = pl.family == FAM_BLOCK_NORM_GRAD;
+    const int norms = a.post + a.pre;
+    const bool sums = grad && norm_sums(a).count() > 0;
+    *reductions = norms * (a.layer && !grad ? 2 : 1) + (sums ? 1 : 0);
+    const size_t by_row = grad ? 1 + size_t(a.branch) : pl.outputs.size();
+    for (size_t k = 0; k < pl.outputs.size(); ++k) {
+      if (k >= by_row) put(k, pl.outputs[k].elements, kNormJoinThreads);
+      else if (norms) put(k, a.rows, row_threads(a.shape));
+      else put(k, pl.outputs[k].elements, 1);
+    }
+  } else {
+    const BiasSoftmaxArgs& a = pl.bias;
+    const bool grad = pl.family == FAM_BIAS_SOFTMAX_GRAD;
+    *reductions = grad ? 2 : 1;
+    const uint64_t rows = a.batch * a.heads * a.queries;
+    put(0, rows, row_threads(a.shape));
+    if (grad) put(1, pl.outputs[1].elements, kBiasJoinThreads);
+    else put(1, rows, row_threads(a.shape));
+  }
+  return groups;
+}
+std::string block_lowering(const ask_b200_plan& pl) {
+  int reductions = 0;
+  const std::vector<OutputGroup> groups = block_groups(pl, &reductions);
+  size_t empty = 0, shared = 0;
+  for (const PortInfo& p : pl.outputs) empty += p.elements == 0;
+  for (const OutputGroup& g : groups) shared += g.threads > 1;
+  std::ostringstream o;
+  o << "{\"statistics_stage\":\"cuda_lowering\",\"kernel_count\":" << pl.launches << ",\"indexing\":\""
+    << (shared ? "cooperative_grid_stride" : "linear_grid_stride") << "\",\"warp_reduction_groups\":" << shared
+    << ",\"output_loop_count\":" << groups.size() << ",\"input_load_count\":" << pl.inputs.size()
+    << ",\"reduction_loop_count\":" << reductions << ",\"zero_element_outputs\":" << empty
+    << ",\"temporary_buffer_count\":0,\"scratch_bytes\":" << pl.scratch << ",\"groups\":[";
+  for (size_t g = 0; g < groups.size(); ++g) {
+    o << (g ? "," : "") << "{\"outputs\":[";
+    for (size_t k = 0; k < groups[g].outputs.size(); ++k) o << (k ? "," : "") << groups[g].outputs[k];
+    o << "],\"element_count\":" << groups[g].count << ",\"threads_per_output\":" << groups[g].threads << "}";
+  }
+  o << "],\"bool_storage\":\"one-byte-zero-or-one\",\"cast_semantics\":\"rne-saturating-fptosi-nan-zero-v1\","
+    << "\"kernel\":\"" << pl.kernel << "\",\"strategy\":\"" << kFamilyNames[pl.family] << "\"}";
+  return o.str();
+}
+
 // The diagnostics the reference's CUDA lowering reports for a step
 // (lib/Lowering/CUDA.cpp:408-417, "cuda_lowering"), for the kernels this plan
 // launches: the same fields with the same meaning, plus the plan's strategy.
@@ -1149,7 +1216,8 @@ void build_bias_softmax(ask_b200_plan& pl, const json::Value& r, bool grad) {
 // reduction of a step folds in the same pass); input_load_count counts input
 // ports, each read once per element.  pre_copy names the step's base input.
 std::string cuda_lowering(const ask_b200_plan& pl, long pre_copy_input) {
-  const bool reduce = pl.family == FAM_REDUCE, softmax = row_family(pl.family);
+  if (pl.family > FAM_SOFTMAX) return block_lowering(pl);
+  const bool reduce = pl.family == FAM_REDUCE, softmax = pl.family == FAM_SOFTMAX;
   const bool warp = (reduce && !pl.views && pl.strategy == RS_WARP_ROW) || softmax;
   const int block = pl.sm_step ? pl.block : pl.family == FAM_ELEMENTWISE ? kEwThreads : reduce ? kRedThreads
                   : softmax ? pl.block : 256;
@@ -1161,7 +1229,7 @@ std::string cuda_lowering(const ask_b200_plan& pl, long pre_copy_input) {
   }
   uint64_t count = pl.outputs.empty() ? 0 : pl.outputs[0].elements;
   if (pl.family == FAM_SCATTER && pl.inputs.size() > 2) count = pl.inputs[2].elements;
-  if (pl.family == FAM_SOFTMAX) count = pl.sm.rows;
+  if (softmax) count = pl.sm.rows;
   uint64_t per_output = warp ? (softmax || pl.sm_step ? uint64_t(pl.block) : 32) : 1;
   if (reduce && !pl.views && pl.strategy == RS_SPLIT) per_output = uint64_t(pl.grid) * uint64_t(block);
   const char* strat[] = {"warp_row", "column", "split"};

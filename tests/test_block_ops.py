@@ -191,3 +191,36 @@ def test_whole_units_end_inside_the_scores(dtype, make):
             for r in range(rows):
                 end = -(-(r + 1) * keys // v) * v  # of the row's last unit, in elements
                 assert (r < whole) == (end <= rows * keys and keys > 0), (keys, rows, r)
+
+
+def test_lowering_report_of_the_block_families():
+    """cuda_lowering says what the kernels do: dropout is a map; rows are reduced by their teams, sums over rows are a
+    group of their own."""
+    def report(recipe):
+        return ask_b200.Plan(recipe, -1).describe()["cuda_lowering"]
+
+    r = report(R.dropout("bf16", 1001, 0.1, residual=True))
+    assert (r["indexing"], r["warp_reduction_groups"], r["reduction_loop_count"], r["output_loop_count"]) == (
+        "linear_grid_stride", 0, 0, 1)
+    assert r["groups"] == [{"outputs": [0], "element_count": 1001, "threads_per_output": 1}] and r["input_load_count"] == 3
+    assert r["strategy"] == "dropout"
+    # rows of 40 go to teams of 4 lanes, rows of 4096 to 256 threads, of 32768 to four CTAs of 512
+    for cols, threads in [(40, 4), (4096, 256), (32768, 2048)]:
+        r = report(R.block_norm("bf16", 12, cols, norm="layer", gate_groups=3))
+        assert (r["indexing"], r["warp_reduction_groups"], r["reduction_loop_count"]) == ("cooperative_grid_stride", 1, 4)
+        assert r["groups"] == [{"outputs": [0, 1, 2, 3], "element_count": 12, "threads_per_output": threads}]
+    r = report(R.block_norm("f32", 5, 7, post=False, pre=False, gate_groups=1))
+    assert (r["indexing"], r["reduction_loop_count"]) == ("linear_grid_stride", 0)
+    assert r["groups"] == [{"outputs": [0], "element_count": 35, "threads_per_output": 1}]
+    r = report(R.block_norm_grad("bf16", 12, 40, gate_groups=3))
+    assert (r["warp_reduction_groups"], r["reduction_loop_count"], r["kernel_count"]) == (4, 3, 2)
+    assert [(g["outputs"], g["element_count"]) for g in r["groups"]] == [([0, 1], 12), ([2], 40), ([3], 120), ([4], 40)]
+    r = report(R.block_norm_grad("f32", 0, 7))
+    assert r["zero_element_outputs"] == 2 and [g["outputs"] for g in r["groups"]] == [[2, 3]]
+    r = report(R.bias_softmax("f16", 2, 3, 5, 256, [1, 2]))
+    assert [(g["outputs"], g["element_count"]) for g in r["groups"]] == [([0, 1], 30)] and r["reduction_loop_count"] == 1
+    assert r["groups"][0]["threads_per_output"] == ask_b200.Plan(R.bias_softmax("f16", 2, 3, 5, 256, [1, 2]), -1).describe()[
+        "launch"]["block"][0]
+    r = report(R.bias_softmax_grad("f16", 2, 3, 5, 256, [1, 2]))
+    assert [(g["outputs"], g["element_count"]) for g in r["groups"]] == [([0], 30), ([1], 18)]
+    assert r["reduction_loop_count"] == 2
