@@ -224,3 +224,14 @@ def test_lowering_report_of_the_block_families():
     r = report(R.bias_softmax_grad("f16", 2, 3, 5, 256, [1, 2]))
     assert [(g["outputs"], g["element_count"]) for g in r["groups"]] == [([0], 30), ([1], 18)]
     assert r["reduction_loop_count"] == 2
+
+
+def test_steps_that_advance_the_offset_share_no_block():
+    """An element count that is no multiple of 4 leaves words of its last block over: the next step starts behind it."""
+    for n in (1, 4, 1001, 1002, 1003, 1004):
+        step = (n + 3) // 4
+        blocks = ref.philox_words(5, 7, 0, 4 * step).reshape(-1, 4)
+        after = ref.philox_words(5, 7 + step, 0, 4 * step).reshape(-1, 4)
+        assert not (blocks[:, None] == after[None]).all(2).any()
+        if n % 4:  # whole division would draw the last block twice
+            assert np.array_equal(ref.philox_words(5, 7 + n // 4, 0, 4), blocks[-1])
