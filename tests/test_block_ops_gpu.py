@@ -616,6 +616,24 @@ def test_gradients_are_deterministic_on_any_stream(device):
             assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(first, again))
 
 
+def test_gradients_on_another_stream_after_their_buffers(device):
+    """As above with the streams in order: outputs and scratch are filled before the other stream starts, and the
+    default stream is kept busy with other buffers while it works."""
+    for recipe, ins in grad_calls():
+        first = launch(recipe, ins)
+        plan = ask_b200.Plan(recipe, device=0)
+        side, busy = torch.cuda.Stream(), torch.zeros(1 << 26, device="cuda")
+        for _ in range(3):
+            outs = [torch.full_like(t, 77) for t in first]
+            scratch = torch.full((plan.scratch_bytes,), 0xA5, dtype=torch.uint8, device="cuda")
+            side.wait_stream(torch.cuda.current_stream())
+            busy += 1
+            plan.launch(ins, outs, scratch, side)
+            torch.cuda.current_stream().wait_stream(side)
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(first, outs))
+        torch.cuda.synchronize()
+
+
 def test_graph_replay_draws_new_masks(device):
     n = 10_000
     x, seed = torch.ones(n, device="cuda"), dev(np.array([1, 0]), "i64")
