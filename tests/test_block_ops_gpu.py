@@ -510,6 +510,13 @@ def test_bias_softmax_gradient_of_rows_far_from_zero(device, dtype, low, step, s
     close(host(dt, want.shape), want, (2 * ref.C + ref.C + shape[0] * shape[2]) * ref.U * wantmag + 2.0 ** -100, "dtable")
 
 
+@pytest.mark.parametrize("dtype,low,step", [("f32", -1e6, 0.25), ("f16", -65504.0, 0.0),
+                                            ("bf16", -3.3895e38, 0.0)])
+def test_bias_softmax_gradient_of_long_rows_far_from_zero(device, dtype, low, step):
+    """The same over a cluster of CTAs, whose sums meet in distributed shared memory."""
+    test_bias_softmax_gradient_of_rows_far_from_zero(device, dtype, low, step, (1, 2, 3, 30000))
+
+
 @pytest.mark.parametrize("keys", [40, 45, 700])
 def test_bias_softmax_gradient_overflow_stays_out_of_masked_places(device, keys):
     """Rows whose sums overflow once the dropout's scale is on them (three of five keys kept): masked keys still get zeros, buckets that only they
