@@ -199,8 +199,8 @@ __device__ __forceinline__ uint4 act_narrow2(const uint64_t* v) {
   return act_narrow<T>(f);
 }
 
-// V parameters (weights, gates) of run-time type starting at column c: read
-// again for every row, so they stay in L1 or L2.
+// V parameters (weights, gates, a bias table's entries) of run-time type starting
+// at column c: read once for many rows and kept in shared memory by the callers.
 template <int V>
 __device__ __forceinline__ void param_load(const void* p, int type, uint64_t c, float* v) {
   if constexpr (V == 1) {

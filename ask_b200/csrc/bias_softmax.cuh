@@ -22,8 +22,8 @@
 //
 // Rows start anywhere (any number of keys): a row is read and written in the
 // tensor's own aligned 16-byte units, whose first and last may hold elements of
-// the neighbouring rows; those are masked, and only such cut units are stored
-// element by element.  Units without a visible key are not read.  The next row's
+// the neighbouring rows; those are masked, and only such cut units are stored in
+// parts (by words, and halves at either end).  Units without a visible key are not read.  The next row's
 // units are on their way (cp.async into words that only their own thread reads)
 // while this row is worked on.
 //
@@ -37,8 +37,8 @@
 // of a scheduler's share of HBM; they take about 20 instructions, 8 clocks of ex2
 // among them, and with dropout the generator's 21 clocks more.  bf16 [8, 16, 1024, 1024]: 95 us full
 // and without dropout (5.6 TB/s), 177 us with dropout and ragged lengths;
-// gradient 148 and 233 us.  Rows that are not whole units add masks, cut
-// stores and a unit more a row (1021 keys: 262 us).
+// gradient 145 and 234 us.  Rows that are not whole units add masks, cut
+// stores and a unit more a row (1021 keys: 264 us).
 #pragma once
 
 #include <cuda_runtime.h>

@@ -4,10 +4,12 @@
 // Bound: HBM, 2 (3 with a residual) elements moved for each one computed; the
 // generator's products (philox.cuh) take about as long as HBM needs for 2-byte
 // elements and half as long as for 4-byte ones, so the next units' loads are
-// issued before this one's integer work.  2^27 bf16 elements take 115 us
-// (4.7 TB/s; the copy alone 82, the generator alone 76: both keep the issue
-// slots busy, so they add in part), 2^26 f32 elements 84.6 us (6.35 TB/s),
-// 17,000,051 of them with a residual 32.5 us (6.3 TB/s).
+// issued before this one's integer work.  2^27 bf16 elements take 120 us
+// (4.5 TB/s; the copy alone 82, the generator alone 76).  Nothing is full then:
+// issue slots 54%, the busiest pipe (widening products) 64%, DRAM below that; four
+// warps a scheduler, which is what the registers leave, wait for the generator's
+// fixed latencies.  2^26 f32 elements take 84.7 us (6.3 TB/s), 17,000,051 of them
+// with a residual 32.7 us (6.2 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

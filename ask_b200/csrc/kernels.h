@@ -236,7 +236,7 @@ struct NormArgs {
   float *dw_post, *db_post, *dgate, *dw_pre, *db_pre;
   float* partial;  // [sum kinds][groups * chunks][cols]
   uint64_t rows, rows_per_group;
-  uint32_t cols, groups, chunks;  // chunks of a group's rows, one team each (gradient)
+  uint32_t cols, groups, chunks;  // chunks of a group's rows, one CTA or cluster each (gradient)
   float alpha, eps;
   int type, ptype;
   int branch, post, pre, layer, bias, gated;

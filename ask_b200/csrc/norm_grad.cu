@@ -10,9 +10,10 @@
 // weight's.  A CTA keeps the sums of its rows' columns in registers, leaves them
 // once in scratch, and a second kernel joins the CTAs' sums in order: results do
 // not depend on the order of execution.  What hhat and yhat hold where there is no
-// column meets du = 0 and c = 0.  bf16 [32768, 4096] takes 314 us with
-// dropout (5.1 TB/s) and 268 without; f16 [4099, 1000] layer norms 28-31 us,
-// mostly the latency of two dependent kernels.
+// column meets du = 0 and c = 0.  bf16 [32768, 4096] takes 338 us with
+// dropout (4.8 TB/s) and 268 without; f16 [4099, 1000] layer norms 29.6 us: the
+// latency of two dependent kernels, the join of 148 places 9 us of it.  Forms for
+// layer norms or biases spill up to 340 bytes a thread at 128 registers, f32 by words most.
 #include "norm_rows.cuh"
 
 namespace askb {

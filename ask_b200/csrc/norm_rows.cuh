@@ -17,12 +17,13 @@
 // holds what is on its way.  Its parameters lie beside them in shared memory for
 // all of its rows.  Arithmetic runs on f32 pairs.  (Rows prefetched into
 // registers and parameters reloaded for each row took 446 us where this takes
-// 231, the gradient 831 where it takes 314.)
+// 243, the gradient 831 where it takes 338.)
 //
 // Bound: HBM, four tensors forward and six for the gradient, up to 6400
 // columns without dropout (bf16 [32768, 4096]: 188 us = 5.7 TB/s, gradient 268 us =
-// 6.0 TB/s); with dropout the generator's products share the issue slots (231 and
-// 314 us).  Wider rows have one team an SM, whose loads wait while it reduces
+// 6.0 TB/s); with dropout the generator's latencies add to it (243 and 338 us; 231
+// and 314 where the same kernel runs back to back, as both sides did in the
+// comparisons below and in the kernels' files).  Wider rows have one team an SM, whose loads wait while it reduces
 // (8192 columns: 161 us for half the elements, gradient 206), and those over a
 // cluster wait for its barriers (16384: 238 and 284).
 #pragma once

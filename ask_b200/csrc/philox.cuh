@@ -53,7 +53,7 @@ static __device__ __noinline__ Philox philox4x32_10_call(uint32_t c0, uint32_t c
 // of the loop (DropRun): counter word 2 is the site's, word 1 changes once in
 // 2^34 elements, so of the first round only lo(b)'s product is left, and of
 // the second one product; and block b + 1 adds the multiplier to block b's first
-// product.  That leaves 17 or 18 products of 20; the tensor takes 115 us with
+// product.  That leaves 17 or 18 products of 20; the tensor takes 120 us with
 // its memory traffic (dropout_kernels.cu).  Products by f64 multiply-adds
 // (88-91 us for the generator alone against 76) and a comparison by a widening
 // multiply-add (157 against 134 us for the whole kernel then) were slower.  A
